@@ -33,6 +33,9 @@ AGM_FLAG_BWD_PAIR = 0x20
 AGM_FLAG_NO_FOLD = 0x40
 AGM_FLAG_DECODE_TILES = 0x80
 AGM_FLAG_NO_FRONT = 0x100
+AGM_ROUTE_SOFTMAX, AGM_ROUTE_SIGMOID = 0, 1
+AGM_ROUTE_MAX_EXPERTS, AGM_ROUTE_MAX_TOPK = 512, 32
+AGM_FP8_AUTO, AGM_FP8_ROWS, AGM_FP8_WEIGHTS = 0, 1, 2
 AGM_CODEC_PLAIN, AGM_CODEC_INT8, AGM_CODEC_INT8_ROWWISE = 0, 1, 2
 AGM_APPLY_COPY, AGM_APPLY_LERP, AGM_APPLY_ADD = 0, 1, 2
 
@@ -105,6 +108,15 @@ SIGNATURES = {
     "agm_moe_aux_saved_bytes": (_SZ, [_I64, _I, _I]),
     "agm_moe_aux_backward_workspace_bytes": (_SZ, [_I64, _I, _I]),
     "agm_moe_aux_forward": (_I, [_P, _I, _I64, _I, _I, _P, ctypes.c_double, ctypes.c_double, _P, _P, _SZ, _I, _P]),
+    "agm_route_experts": (_I, [_P, _I, _I64, _I, _I, _I, _P, _I, _I, _I, ctypes.c_float, _P, _P, _P]),
+    "agm_route_experts_backward": (_I, [_P, _P, _I, _I64, _I, _I, _P, _I, _I, ctypes.c_float, _P, _P]),
+    "agm_fp8_scale_bytes": (_SZ, [_I64, _I]),
+    "agm_quantize_fp8": (_I, [_P, _I, _I64, _I, _P, _P, _P]),
+    "agm_quantize_fp8_weight": (_I, [_P, _I, _I64, _I, _I, _P, _P, _P]),
+    "agm_dequantize_fp8": (_I, [_P, _P, _I64, _I64, _I, _I, _P, _P]),
+    "agm_grouped_gemm_fp8": (_I, [_P, _P, _I64, _P, _P, _P, _I, _I, _I, _P, _P, _I, _I, _P, _I, _P, _P, _P]),
+    "agm_moe_experts_fp8_workspace_bytes": (_SZ, [_I64, _I, _I, _I, _I]),
+    "agm_moe_experts_fp8": (_I, [_P, _I, _I64, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "agm_moe_aux_backward": (_I, [_P, _P, _I, _I64, _I, _I, _P, _SZ, _P, _P, _SZ, _I, _P]),
 }
 

@@ -1,0 +1,540 @@
+// Block-scaled e4m3: quantisation of rows and of weights, the inverse, and the
+// expert dispatch and weighted sum around the 8-bit grouped products.
+//
+// All of these move memory and are bound by it. A lane owns 16 consecutive
+// elements (one 16-byte store of e4m3), 8 lanes a block of 128, a warp 512
+// columns of a row, whose four scales are one 32-bit word of the row's scale
+// tile.
+#include <algorithm>
+
+#include "fp8.cuh"
+#include "kernels.h"
+
+namespace agm {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kTokBlk = AGM_DISPATCH_BLOCK;
+
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, float (&v)[16]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 f = __ldcs(reinterpret_cast<const float4*>(p) + i);
+      v[4 * i] = f.x;
+      v[4 * i + 1] = f.y;
+      v[4 * i + 2] = f.z;
+      v[4 * i + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float f[8];
+      unpack8<T>(__ldcs(reinterpret_cast<const uint4*>(p) + i), f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[8 * i + j] = f[j];
+    }
+  }
+}
+
+__device__ __forceinline__ float amax16(const float (&v)[16]) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = fmaxf(m, finite_abs(v[i]));
+  return m;
+}
+
+__device__ __forceinline__ uint4 encode16(const float (&v)[16], float inv) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = pack_e4m3x4(inf_to_nan(v[4 * i]) * inv, inf_to_nan(v[4 * i + 1]) * inv, inf_to_nan(v[4 * i + 2]) * inv,
+                       inf_to_nan(v[4 * i + 3]) * inv);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Quantises the lane's 16 elements of 512 columns of a row; *word is the row's
+// scale word (in every lane).
+__device__ __forceinline__ uint4 encode_unit(const float (&v)[16], int lane, uint32_t& word) {
+  float m = amax16(v);
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const uint32_t byte = scale_byte(m);
+  uint32_t w = byte << (8 * (lane >> 3));
+  w |= __shfl_xor_sync(0xffffffffu, w, 8);
+  w |= __shfl_xor_sync(0xffffffffu, w, 16);
+  word = w;
+  return encode16(v, inv_scale(byte));
+}
+
+template <typename T>
+__device__ __forceinline__ void load_unit(const T* x, int64_t row, int k4, int width, int lane, float (&v)[16]) {
+  const int c = k4 * 512 + lane * 16;
+  if (c < width) {
+    load16<T>(x + row * width + c, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = 0.f;
+  }
+}
+
+// One warp per (row, 512 columns); rows up to the next multiple of 128 get a
+// scale word only, so that whole scale tiles are defined.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int width, int width_k4, uint8_t* __restrict__ q,
+                         uint8_t* __restrict__ scales) {
+  const int lane = lane_id();
+  const int64_t units = (rows + 127) / 128 * 128 * width_k4;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + warp_id(); u < units; u += step) {
+    const int64_t row = u / width_k4;
+    const int k4 = static_cast<int>(u - row * width_k4);
+    uint32_t word = 0;
+    if (row < rows) {
+      float v[16];
+      load_unit<T>(x, row, k4, width, lane, v);
+      const uint4 o = encode_unit(v, lane, word);
+      const int c = k4 * 512 + lane * 16;
+      if (c < width) *reinterpret_cast<uint4*>(q + row * width + c) = o;
+    }
+    if (lane == 0) *reinterpret_cast<uint32_t*>(scales + scale_word_offset(row, k4, width_k4)) = word;
+  }
+}
+
+// One CTA per 128 x 128 block: 8 lanes hold a row of the block, 4 passes of 32
+// rows stay in registers between the maximum and the rounding.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    quantize_weight_kernel(const T* __restrict__ w, int n, int width, int width_k4, uint8_t* __restrict__ q,
+                           uint8_t* __restrict__ scales) {
+  __shared__ float max_s[kWarps];
+  const int kb = blockIdx.x, nb = blockIdx.y;
+  const int tiles = gridDim.y;
+  const int64_t g = blockIdx.z;
+  const int lane = lane_id(), sub = threadIdx.x & 7, r0 = threadIdx.x >> 3;
+  const int c = kb * 128 + sub * 16;
+  const int64_t base = g * n;
+  float v[4][16], m = 0.f;
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int r = nb * 128 + p * 32 + r0;
+    if (r < n && c < width) {
+      load16<T>(w + (base + r) * width + c, v[p]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[p][i] = 0.f;
+    }
+    m = fmaxf(m, amax16(v[p]));
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) max_s[warp_id()] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) m = fmaxf(m, max_s[i]);
+  const uint32_t byte = scale_byte(m);
+  const float inv = inv_scale(byte);
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int r = nb * 128 + p * 32 + r0;
+    if (r < n && c < width) *reinterpret_cast<uint4*>(q + (base + r) * width + c) = encode16(v[p], inv);
+  }
+  // Every row of the tile gets the block's byte; the last block also clears
+  // the bytes of the K blocks that do not exist.
+  const int blocks = (width + 127) / 128;
+  if (threadIdx.x < 128) {
+    uint8_t* tile = scales + (g * tiles + nb) * static_cast<int64_t>(width_k4) * kScaleTile;
+    const int64_t at = scale_word_offset(threadIdx.x, kb >> 2, width_k4) + (kb & 3);
+    tile[at] = static_cast<uint8_t>(byte);
+    if (kb == blocks - 1)
+      for (int b = (kb & 3) + 1; b < 4; ++b) tile[at - (kb & 3) + b] = 0;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales, int64_t groups, int64_t rows,
+                      int width, int width_k4, T* __restrict__ out) {
+  const int lane = lane_id();
+  const int64_t tile_rows = (rows + 127) / 128 * 128;
+  const int64_t units = groups * rows * width_k4;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + warp_id(); u < units; u += step) {
+    const int64_t gr = u / width_k4;
+    const int k4 = static_cast<int>(u - gr * width_k4);
+    const int64_t g = gr / rows;
+    const int64_t r = gr - g * rows;
+    const int c = k4 * 512 + lane * 16;
+    if (c >= width) continue;
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(scales + scale_word_offset(g * tile_rows + r, k4, width_k4));
+    const float s = scale_value((word >> (8 * (lane >> 3))) & 0xffu);
+    const uint4 b = __ldcs(reinterpret_cast<const uint4*>(q + gr * width + c));
+    const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = unpack_e4m3x2(bw[i >> 1] >> (16 * (i & 1)));
+      v[2 * i] = f.x * s;
+      v[2 * i + 1] = f.y * s;
+    }
+    T* o = out + gr * width + c;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        reinterpret_cast<float4*>(o)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        reinterpret_cast<uint4*>(o)[i] = make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
+                                                    pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Dispatch
+// ---------------------------------------------------------------------------
+// Quantises token `tok`'s row once and writes it to the k rows dest[0 .. k).
+template <typename T>
+__device__ __forceinline__ void scatter_row(const Fp8Dispatch& a, int64_t tok, const int32_t* dest, int width_k4,
+                                            int lane) {
+  for (int k4 = 0; k4 < width_k4; ++k4) {
+    float v[16];
+    load_unit<T>(static_cast<const T*>(a.x), tok, k4, a.d, lane, v);
+    uint32_t word;
+    const uint4 o = encode_unit(v, lane, word);
+    const int c = k4 * 512 + lane * 16;
+    for (int r = 0; r < a.k; ++r) {
+      const int64_t row = dest[r];
+      if (row < 0) continue;
+      if (c < a.d) *reinterpret_cast<uint4*>(a.q + row * a.d + c) = o;
+      if (lane == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word_offset(row, k4, width_k4)) = word;
+    }
+  }
+}
+
+__device__ __forceinline__ int pad_rows(int count) { return (count + AGM_TILE_M - 1) / AGM_TILE_M * AGM_TILE_M; }
+
+// Exclusive prefix of the padded counts in count_s over E <= 512 experts, by
+// one warp: start_s[E + 1].
+__device__ __forceinline__ void padded_prefix(const int* count_s, int E, int* start_s, int lane) {
+  int carry = 0;
+  for (int e0 = 0; e0 < E; e0 += 32) {
+    const int e = e0 + lane;
+    const int v = e < E ? pad_rows(count_s[e]) : 0;
+    int incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
+    }
+    if (e < E) start_s[e] = carry + incl - v;
+    carry += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  if (lane == 0) start_s[E] = carry;
+}
+
+// Small batches: every CTA counts all slots by itself and moves its share of
+// the tokens, one launch in all.
+constexpr int kSmallSlots = 2048;
+template <typename T>
+__global__ void __launch_bounds__(kThreads) dispatch_small_kernel(Fp8Dispatch a, int width_k4) {
+  __shared__ int idx_s[kSmallSlots];
+  __shared__ int count_s[AGM_ROUTE_MAX_EXPERTS];
+  __shared__ int start_s[AGM_ROUTE_MAX_EXPERTS + 1];
+  __shared__ int dest_s[kWarps][AGM_ROUTE_MAX_TOPK];
+  const int lane = lane_id(), warp = warp_id();
+  pdl_wait();
+  pdl_trigger();
+  const int slots = static_cast<int>(a.n) * a.k;
+  for (int e = threadIdx.x; e < a.n_experts; e += kThreads) count_s[e] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < slots; i += kThreads) {
+    int e = a.idx[i];
+    if (e < 0 || e >= a.n_experts) e = -1;
+    idx_s[i] = e;
+    if (e >= 0) atomicAdd(&count_s[e], 1);
+  }
+  __syncthreads();
+  if (warp == 0) padded_prefix(count_s, a.n_experts, start_s, lane);
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    for (int e = threadIdx.x; e < a.n_experts; e += kThreads) {
+      a.counts[e] = count_s[e];
+      a.seg_start[e] = start_s[e];
+    }
+    if (threadIdx.x == 0) {
+      a.seg_start[a.n_experts] = start_s[a.n_experts];
+      if (start_s[a.n_experts] > a.max_rows) raise_error(a.err, kErrRowOverflow);
+    }
+  }
+  for (int t = blockIdx.x * kWarps + warp; t < a.n; t += gridDim.x * kWarps) {
+    for (int r = 0; r < a.k; ++r) {
+      const int s = t * a.k + r, e = idx_s[s];
+      int before = 0;
+      for (int i = lane; i < s; i += 32) before += idx_s[i] == e;
+      before = __reduce_add_sync(0xffffffffu, before);
+      if (lane == 0) {
+        const int64_t row = e >= 0 ? static_cast<int64_t>(start_s[e]) + before : -1;
+        dest_s[warp][r] = row < a.max_rows ? static_cast<int>(row) : -1;
+        a.row_of[s] = dest_s[warp][r];
+      }
+    }
+    __syncwarp();
+    scatter_row<T>(a, t, dest_s[warp], width_k4, lane);
+    __syncwarp();
+  }
+}
+
+// Large batches, three launches. 1: per-expert counts of every 128 tokens.
+__global__ void __launch_bounds__(kThreads)
+    dispatch_hist_kernel(const int32_t* __restrict__ idx, int64_t slots, int k, int E, int32_t* __restrict__ hist) {
+  __shared__ int count_s[AGM_ROUTE_MAX_EXPERTS];
+  pdl_wait();
+  pdl_trigger();
+  for (int e = threadIdx.x; e < E; e += kThreads) count_s[e] = 0;
+  __syncthreads();
+  const int64_t s0 = static_cast<int64_t>(blockIdx.x) * kTokBlk * k;
+  const int64_t s1 = min(slots, s0 + static_cast<int64_t>(kTokBlk) * k);
+  for (int64_t s = s0 + threadIdx.x; s < s1; s += kThreads) {
+    const int e = idx[s];
+    if (e >= 0 && e < E) atomicAdd(&count_s[e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += kThreads) hist[static_cast<int64_t>(blockIdx.x) * E + e] = count_s[e];
+}
+
+// 2: per expert, the counts of its blocks become offsets in its segment (one
+// warp per expert, in place).
+__global__ void __launch_bounds__(kThreads)
+    dispatch_scan_kernel(int32_t* __restrict__ hist, int n_blocks, int E, int32_t* __restrict__ counts) {
+  constexpr int kUnroll = 8;
+  pdl_wait();
+  pdl_trigger();
+  const int lane = lane_id();
+  const int e = blockIdx.x * kWarps + warp_id();
+  if (e >= E) return;
+  int carry = 0;
+  for (int b0 = 0; b0 < n_blocks; b0 += 32 * kUnroll) {
+    int v[kUnroll];
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      const int b = b0 + 32 * j + lane;
+      v[j] = b < n_blocks ? hist[static_cast<int64_t>(b) * E + e] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      const int b = b0 + 32 * j + lane;
+      int incl = v[j];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+      }
+      if (b < n_blocks) hist[static_cast<int64_t>(b) * E + e] = carry + incl - v[j];
+      carry += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
+  if (lane == 0) counts[e] = carry;
+}
+
+// 3: destinations of a block's slots in slot order, then its rows. Each warp
+// ranks an eighth of the block's slots: matching lanes of 32 slots at a time,
+// on top of the counts of the warps before it.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) dispatch_rows_kernel(Fp8Dispatch a, int width_k4) {
+  __shared__ int start_s[AGM_ROUTE_MAX_EXPERTS + 1];
+  __shared__ int base_s[kWarps][AGM_ROUTE_MAX_EXPERTS];
+  __shared__ int32_t dest_s[kTokBlk * AGM_ROUTE_MAX_TOPK];
+  const int lane = lane_id(), warp = warp_id();
+  const int E = a.n_experts;
+  pdl_wait();
+  pdl_trigger();
+  const int64_t tok0 = static_cast<int64_t>(blockIdx.x) * kTokBlk;
+  const int toks = static_cast<int>(min(static_cast<int64_t>(kTokBlk), a.n - tok0));
+  const int slots = toks * a.k;
+  const int per_warp = (slots + kWarps - 1) / kWarps;
+  const int s0 = min(slots, warp * per_warp), s1 = min(slots, s0 + per_warp);
+  const int32_t* idx = a.idx + tok0 * a.k;
+  if (warp == 0) padded_prefix(a.counts, E, start_s, lane);
+  for (int e = lane; e < E; e += 32) base_s[warp][e] = 0;
+  __syncwarp();
+  for (int s = s0 + lane; s < s1; s += 32) {
+    const int e = idx[s];
+    if (e >= 0 && e < E) atomicAdd(&base_s[warp][e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += kThreads) {
+    int at = start_s[e] + a.block_hist[static_cast<int64_t>(blockIdx.x) * E + e];
+    for (int w = 0; w < kWarps; ++w) {
+      const int c = base_s[w][e];
+      base_s[w][e] = at;
+      at += c;
+    }
+    if (blockIdx.x == 0) a.seg_start[e] = start_s[e];
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.seg_start[E] = start_s[E];
+    if (start_s[E] > a.max_rows) raise_error(a.err, kErrRowOverflow);
+  }
+  __syncthreads();
+  for (int b = s0; b < s1; b += 32) {
+    const int s = b + lane;
+    int e = s < s1 ? idx[s] : -1;
+    if (e < 0 || e >= E) e = -1;
+    const uint32_t peers = __match_any_sync(0xffffffffu, e);
+    const int base = e >= 0 ? base_s[warp][e] : 0;
+    __syncwarp();
+    if (s < s1) {
+      const int row = e >= 0 ? base + __popc(peers & ((1u << lane) - 1u)) : -1;
+      dest_s[s] = row < a.max_rows ? row : -1;
+      a.row_of[tok0 * a.k + s] = dest_s[s];
+    }
+    if (e >= 0 && lane == __ffs(peers) - 1) base_s[warp][e] = base + __popc(peers);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int i = warp; i < toks; i += kWarps) scatter_row<T>(a, tok0 + i, dest_s + i * a.k, width_k4, lane);
+}
+
+// ---------------------------------------------------------------------------
+// Weighted sum
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    combine_weighted_kernel(const T* __restrict__ y, const int32_t* __restrict__ row_of,
+                            const float* __restrict__ weights, int64_t n, int nchunk, int k,
+                            const T* __restrict__ residual, T* __restrict__ out) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = lane_id();
+  const uint4* y4 = reinterpret_cast<const uint4*>(y);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + warp_id(); t < n; t += step) {
+    const int my_row = lane < k ? row_of[t * k + lane] : -1;
+    const float my_w = lane < k ? weights[t * k + lane] : 0.f;
+    for (int c = lane; c - lane < nchunk; c += 32) {
+      float acc[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+      if (residual && c < nchunk) unpack8<T>(__ldcs(reinterpret_cast<const uint4*>(residual) + t * nchunk + c), acc);
+      for (int r = 0; r < k; ++r) {
+        const int row = __shfl_sync(0xffffffffu, my_row, r);
+        const float w = __shfl_sync(0xffffffffu, my_w, r);
+        if (row >= 0 && c < nchunk) {
+          float f[8];
+          unpack8<T>(__ldcs(y4 + static_cast<int64_t>(row) * nchunk + c), f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, f[i], acc[i]);
+        }
+      }
+      if (c < nchunk)
+        reinterpret_cast<uint4*>(out)[t * nchunk + c] = make_uint4(pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3]),
+                                                                   pack2<T>(acc[4], acc[5]), pack2<T>(acc[6], acc[7]));
+    }
+  }
+}
+
+unsigned warp_grid(int64_t units, int num_sms) {
+  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((units + kWarps - 1) / kWarps,
+                                                                      static_cast<int64_t>(num_sms) * 8)));
+}
+
+template <typename T>
+cudaError_t dispatch_t(const Fp8Dispatch& a, int num_sms, cudaStream_t stream) {
+  const int width_k4 = scale_k4(a.d);
+  if (a.n * a.k <= kSmallSlots)
+    return launch_kernel(dispatch_small_kernel<T>, dim3(warp_grid(a.n, num_sms)), dim3(kThreads), 0, stream, a, width_k4);
+  const int nb = static_cast<int>((a.n + kTokBlk - 1) / kTokBlk);
+  cudaError_t e = launch_kernel(dispatch_hist_kernel, dim3(nb), dim3(kThreads), 0, stream, a.idx, a.n * a.k, a.k,
+                                a.n_experts, a.block_hist);
+  if (e != cudaSuccess) return e;
+  e = launch_kernel(dispatch_scan_kernel, dim3((a.n_experts + kWarps - 1) / kWarps), dim3(kThreads), 0, stream,
+                    a.block_hist, nb, a.n_experts, a.counts);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(dispatch_rows_kernel<T>, dim3(nb), dim3(kThreads), 0, stream, a, width_k4);
+}
+
+}  // namespace
+
+cudaError_t quantize_fp8_rows(int dtype, const void* x, int64_t rows, int width, void* q, void* scales, int num_sms,
+                              cudaStream_t stream) {
+  const int k4 = scale_k4(width);
+  const unsigned grid = warp_grid((rows + 127) / 128 * 128 * k4, num_sms);
+  uint8_t* qb = static_cast<uint8_t*>(q);
+  uint8_t* sb = static_cast<uint8_t*>(scales);
+  switch (dtype) {
+    case AGM_F32:
+      quantize_rows_kernel<float><<<grid, kThreads, 0, stream>>>(static_cast<const float*>(x), rows, width, k4, qb, sb);
+      break;
+    case AGM_BF16:
+      quantize_rows_kernel<__nv_bfloat16>
+          <<<grid, kThreads, 0, stream>>>(static_cast<const __nv_bfloat16*>(x), rows, width, k4, qb, sb);
+      break;
+    default:
+      quantize_rows_kernel<__half><<<grid, kThreads, 0, stream>>>(static_cast<const __half*>(x), rows, width, k4, qb, sb);
+  }
+  return cudaGetLastError();
+}
+
+cudaError_t quantize_fp8_weight(int dtype, const void* w, int64_t groups, int n, int width, void* q, void* scales,
+                                cudaStream_t stream) {
+  const int k4 = scale_k4(width);
+  const dim3 grid((width + 127) / 128, (n + 127) / 128, static_cast<unsigned>(groups));
+  uint8_t* qb = static_cast<uint8_t*>(q);
+  uint8_t* sb = static_cast<uint8_t*>(scales);
+  switch (dtype) {
+    case AGM_F32:
+      quantize_weight_kernel<float><<<grid, kThreads, 0, stream>>>(static_cast<const float*>(w), n, width, k4, qb, sb);
+      break;
+    case AGM_BF16:
+      quantize_weight_kernel<__nv_bfloat16>
+          <<<grid, kThreads, 0, stream>>>(static_cast<const __nv_bfloat16*>(w), n, width, k4, qb, sb);
+      break;
+    default:
+      quantize_weight_kernel<__half><<<grid, kThreads, 0, stream>>>(static_cast<const __half*>(w), n, width, k4, qb, sb);
+  }
+  return cudaGetLastError();
+}
+
+cudaError_t dequantize_fp8(int dtype, const void* q, const void* scales, int64_t groups, int64_t rows, int width,
+                           void* out, int num_sms, cudaStream_t stream) {
+  const int k4 = scale_k4(width);
+  const unsigned grid = warp_grid(groups * rows * k4, num_sms);
+  const uint8_t* qb = static_cast<const uint8_t*>(q);
+  const uint8_t* sb = static_cast<const uint8_t*>(scales);
+  switch (dtype) {
+    case AGM_F32:
+      dequantize_kernel<float><<<grid, kThreads, 0, stream>>>(qb, sb, groups, rows, width, k4, static_cast<float*>(out));
+      break;
+    case AGM_BF16:
+      dequantize_kernel<__nv_bfloat16>
+          <<<grid, kThreads, 0, stream>>>(qb, sb, groups, rows, width, k4, static_cast<__nv_bfloat16*>(out));
+      break;
+    default:
+      dequantize_kernel<__half><<<grid, kThreads, 0, stream>>>(qb, sb, groups, rows, width, k4, static_cast<__half*>(out));
+  }
+  return cudaGetLastError();
+}
+
+cudaError_t dispatch_fp8(int dtype, const Fp8Dispatch& a, int num_sms, cudaStream_t stream) {
+  return dtype == AGM_BF16 ? dispatch_t<__nv_bfloat16>(a, num_sms, stream) : dispatch_t<__half>(a, num_sms, stream);
+}
+
+cudaError_t combine_weighted(int dtype, const void* y, const int32_t* row_of, const float* weights, int64_t n, int d,
+                             int k, const void* residual, void* out, int num_sms, cudaStream_t stream) {
+  const dim3 grid(warp_grid(n, num_sms));
+  const int nchunk = d / 8;
+  if (dtype == AGM_BF16)
+    return launch_kernel(combine_weighted_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, stream,
+                         static_cast<const __nv_bfloat16*>(y), row_of, weights, n, nchunk, k,
+                         static_cast<const __nv_bfloat16*>(residual), static_cast<__nv_bfloat16*>(out));
+  return launch_kernel(combine_weighted_kernel<__half>, grid, dim3(kThreads), 0, stream, static_cast<const __half*>(y),
+                       row_of, weights, n, nchunk, k, static_cast<const __half*>(residual), static_cast<__half*>(out));
+}
+
+}  // namespace agm

@@ -420,7 +420,7 @@ static EncodeTiledFn get_encode_fn() {
 
 // 2-D/3-D row-major tensor of 16-bit elements: dims innermost first.
 bool encode_tmap(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
-                        const uint32_t* box, CUtensorMapDataType dt) {
+                        const uint32_t* box, CUtensorMapDataType dt, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn || rank < 1 || rank > 5) return false;
   cuuint64_t gdim[5], gstr[4];
@@ -432,7 +432,7 @@ bool encode_tmap(CUtensorMap* m, const void* base, int rank, const uint64_t* dim
   }
   for (int i = 0; i < rank - 1; ++i) gstr[i] = strides_bytes[i];
   CUresult r = fn(m, dt, rank, const_cast<void*>(base), gdim, gstr, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
 }
 

@@ -177,10 +177,10 @@ struct EpRows {
   }
 };
 
-// Tiled TMA descriptor (128-byte swizzle, zero OOB fill) for a row-major
+// Tiled TMA descriptor (128-byte swizzle unless given, zero OOB fill) for a row-major
 // tensor of rank 1 to 5; dims and box innermost first, strides in bytes.
 bool encode_tmap(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
-                 const uint32_t* box, CUtensorMapDataType dt);
+                 const uint32_t* box, CUtensorMapDataType dt, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 
 // Set the message returned by agm_last_error() (thread-local).
 void set_last_error(const std::string& msg);
@@ -289,5 +289,75 @@ cudaError_t grouped_gemm_wgrad_pair(int dtype, bool out_f32, const void* dc, con
 cudaError_t combine(int dtype, const void* y, const int32_t* row_of, const void* gates, int64_t n, int d, int k,
                     const void* shared_y, int n_shared, int64_t shared_stride, const void* residual, void* out,
                     int num_sms, cudaStream_t stream);
+
+// General expert routing (route.cu).
+struct RouteArgs {
+  int64_t n;
+  int n_experts;
+  int k;
+  int score;          // AGM_ROUTE_SOFTMAX or AGM_ROUTE_SIGMOID
+  int n_groups;
+  int top_groups;
+  int renormalize;
+  float scale;
+  const float* bias;  // [n_experts] or nullptr
+};
+cudaError_t route_experts(int dtype, const void* logits, const RouteArgs& a, int32_t* idx, float* weights, int num_sms,
+                          cudaStream_t stream);
+cudaError_t route_experts_backward(int dtype, const float* dw, const void* logits, const int32_t* idx,
+                                   const RouteArgs& a, void* dl, int num_sms, cudaStream_t stream);
+
+// Block-scaled e4m3 (fp8.cu; the format is described in fp8.cuh).
+cudaError_t quantize_fp8_rows(int dtype, const void* x, int64_t rows, int width, void* q, void* scales, int num_sms,
+                              cudaStream_t stream);
+cudaError_t quantize_fp8_weight(int dtype, const void* w, int64_t groups, int n, int width, void* q, void* scales,
+                                cudaStream_t stream);
+cudaError_t dequantize_fp8(int dtype, const void* q, const void* scales, int64_t groups, int64_t rows, int width,
+                           void* out, int num_sms, cudaStream_t stream);
+// Expert dispatch for up to AGM_ROUTE_MAX_EXPERTS experts with the rows
+// quantised on the way: segments padded to 128 rows, in ascending slot order.
+struct Fp8Dispatch {
+  const void* x;        // [n, d]
+  const int32_t* idx;   // [n, k], outside [0, E): slot goes nowhere
+  int64_t n;
+  int d;
+  int k;
+  int n_experts;
+  int64_t max_rows;
+  int32_t* block_hist;  // [ceil(n / 128), E] (large batches)
+  int32_t* counts;      // [E]
+  int32_t* seg_start;   // [E + 1]
+  int32_t* row_of;      // [n, k], -1: nowhere
+  uint8_t* q;           // [max_rows, d]
+  uint8_t* scales;      // scale tiles of q
+  int* err;
+};
+cudaError_t dispatch_fp8(int dtype, const Fp8Dispatch& a, int num_sms, cudaStream_t stream);
+// out[t] = (residual[t] +) sum_r weights[t, r] y[row_of[t, r]], summed in fp32.
+cudaError_t combine_weighted(int dtype, const void* y, const int32_t* row_of, const float* weights, int64_t n, int d,
+                             int k, const void* residual, void* out, int num_sms, cudaStream_t stream);
+// c[r, :] = act(a[r, :] @ w[g]^T + bias[g]) over block-scaled e4m3 (fp8_gemm.cu).
+struct Fp8GemmArgs {
+  const void* a = nullptr;         // e4m3 [a_rows, k]
+  const void* a_scales = nullptr;
+  int64_t a_rows = 0;
+  const void* w = nullptr;         // e4m3 [groups, n, k]
+  const void* w_scales = nullptr;  // scale tiles per group
+  const float* bias = nullptr;     // [groups, n]
+  int groups = 1;
+  int n = 0;
+  int k = 0;
+  // Group g's rows are [seg_start[g], + counts[g]), seg_start multiples of 128
+  // (device arrays); both null: one group over all rows.
+  const int32_t* seg_start = nullptr;
+  const int32_t* counts = nullptr;
+  int64_t live_rows = 0;           // host bound on the sum of the counts
+  bool relu = false;
+  bool zero_pad = false;           // write zeros to a segment's rows behind its count
+  void* c = nullptr;               // [a_rows, n], c_dtype, or e4m3 when c_scales is set
+  void* c_scales = nullptr;
+  int* err = nullptr;
+};
+cudaError_t grouped_gemm_fp8(int c_dtype, const Fp8GemmArgs& args, int mode, int num_sms, cudaStream_t stream);
 
 }  // namespace agm

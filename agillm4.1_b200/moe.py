@@ -182,6 +182,33 @@ def collect_moe_aux(model, aux_coef=0.0, z_coef=0.0):
     return total if total is not None else 0.0
 
 
+class _RouteNode(torch.autograd.Function):
+    """Autograd node of :func:`route_experts`: only the weights carry a
+    gradient, to the logits (the choice and the balance bias have none)."""
+
+    @staticmethod
+    def forward(ctx, logits, bias, top_k, score, n_groups, top_groups, renormalize, scale):
+        idx, weights = ops.route_experts(logits, top_k, score=score, bias=bias, n_groups=n_groups,
+                                         top_groups=top_groups, renormalize=renormalize, scale=scale)
+        ctx.save_for_backward(logits, idx)
+        ctx.options = dict(score=score, renormalize=renormalize, scale=scale)
+        ctx.mark_non_differentiable(idx)
+        return idx, weights
+
+    @staticmethod
+    def backward(ctx, _, dweights):
+        logits, idx = ctx.saved_tensors
+        return (ops.route_experts_backward(dweights.contiguous(), logits, idx, **ctx.options),) + (None,) * 7
+
+
+def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Optional[torch.Tensor] = None,
+                  n_groups: int = 1, top_groups: Optional[int] = None, renormalize: bool = True, scale: float = 1.0):
+    """:func:`ops.route_experts` with autograd: router logits [N, E] ->
+    (idx int32 [N, k], weights fp32 [N, k]), differentiable in the logits."""
+    return _RouteNode.apply(logits.contiguous(), None if bias is None else bias.detach(), top_k, score, n_groups,
+                            top_groups, renormalize, scale)
+
+
 class _B200Forward:
     """Forward of the MoE block on the B200 kernels (mixed into the module classes)."""
 

@@ -10,11 +10,20 @@ of the reference forward (agillm41.py:4389-4431):
 * :func:`grouped_gemm`     expert Linear layers over all segments (4428, 4332-4336)
 * :func:`combine`          gate-weighted `index_add_` + shared experts (4420-4430)
 * :func:`moe_forward`      all of the above in one call, no host sync
+
+General routing and 8-bit experts (beyond the reference's block):
+
+* :func:`route_experts`, :func:`route_experts_backward`   softmax or sigmoid scores of given
+  logits, selection bias, groups, top-k, renormalised and scaled weights
+* :func:`quantize_fp8`, :func:`quantize_fp8_weight`, :func:`dequantize_fp8`   e4m3 with one
+  power-of-two scale per block of 128
+* :func:`grouped_gemm_fp8`  expert Linear layers over such blocks
+* :func:`moe_experts_fp8`   the routed experts of a block, given the routing
 """
 from __future__ import annotations
 
 import ctypes
-from typing import Dict, Optional
+from typing import Dict, NamedTuple, Optional, Union
 
 import torch
 
@@ -542,3 +551,251 @@ def moe_aux_backward(dloss: torch.Tensor, x: torch.Tensor, w_router: torch.Tenso
                                   ptr(ws), ws.numel(), 0, stream_handle(dev))
     check(rc, "agm_moe_aux_backward")
     return dw
+
+
+# ---------------------------------------------------------------------------
+# General routing and block-scaled 8-bit experts
+# ---------------------------------------------------------------------------
+def _call(dev: torch.device, name: str, *args) -> None:
+    """Call a C entry point on ``dev``'s current stream, whichever device is current."""
+    fn = getattr(load(), name)
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, stream_handle(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream_handle(dev))
+    check(rc, name)
+
+
+def _need(what: str, t: torch.Tensor, dtype, shape, dev: torch.device) -> None:
+    """Refuse a tensor that is not of this dtype and shape on this GPU."""
+    if not t.is_cuda:
+        raise _lib.MoEKernelError(f"{what} must be a CUDA tensor: the MoE kernels have no CPU path")
+    if t.device != dev:
+        raise _lib.MoEKernelError(f"{what} is on {t.device}, not on {dev}")
+    if t.dtype != dtype:
+        raise _lib.MoEKernelError(f"{what} must be {dtype}, not {t.dtype}")
+    if t.shape != shape:
+        raise _lib.MoEKernelError(f"{what} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+
+
+def _cuda_matrix(what: str, t: torch.Tensor, dim: int = 2) -> torch.device:
+    if t.dim() != dim:
+        raise _lib.MoEKernelError(f"{what} must have {dim} dimensions, not shape {tuple(t.shape)}")
+    if not t.is_cuda:
+        raise _lib.MoEKernelError(f"{what} must be a CUDA tensor: the MoE kernels have no CPU path")
+    return t.device
+
+
+_SCORES = {"softmax": _lib.AGM_ROUTE_SOFTMAX, "sigmoid": _lib.AGM_ROUTE_SIGMOID}
+
+
+def _score_code(score: str) -> int:
+    try:
+        return _SCORES[score]
+    except KeyError:
+        raise _lib.MoEKernelError(f"score must be 'softmax' or 'sigmoid', not {score!r}") from None
+
+
+def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Optional[torch.Tensor] = None,
+                  n_groups: int = 1, top_groups: Optional[int] = None, renormalize: bool = True, scale: float = 1.0):
+    """Expert routing of router logits [N, E] (E <= 512) -> (idx int32 [N, k], weights fp32 [N, k]).
+
+    s = softmax(logits) over all experts, or sigmoid(logits). The key of the
+    choice is s, plus ``bias`` (fp32 [E], for load balance) when given. With
+    ``n_groups`` > 1 only the ``top_groups`` groups of E / n_groups consecutive
+    experts are kept whose two largest keys have the largest sum. idx holds the
+    top_k (<= 32) largest keys in descending order, ties to the lowest index;
+    weights = scale * s[idx], divided by their sum when ``renormalize``.
+
+    An expert with logit -inf, or whose key is -inf or NaN, is never chosen;
+    a slot left without an expert gets idx -1 and weight 0 (a token routed
+    nowhere is a row of -inf). A row with a NaN logit (+inf too, under softmax)
+    gets NaN weights. The gradient is :func:`route_experts_backward`;
+    :func:`agillm41_b200.route_experts` is the differentiable form."""
+    dev = _cuda_matrix("logits", logits)
+    n, E = logits.shape
+    if bias is not None:
+        _need("bias", bias, torch.float32, (E,), dev)
+    idx = torch.empty(n, top_k, dtype=torch.int32, device=dev)
+    weights = torch.empty(n, top_k, dtype=torch.float32, device=dev)
+    _call(dev, "agm_route_experts", ptr(logits), dtype_code(logits.dtype), n, E, top_k, _score_code(score), ptr(bias),
+          n_groups, n_groups if top_groups is None else top_groups, int(renormalize), float(scale), ptr(idx),
+          ptr(weights))
+    return idx, weights
+
+
+def route_experts_backward(dweights: torch.Tensor, logits: torch.Tensor, idx: torch.Tensor, *, score: str = "softmax",
+                           renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
+    """Gradient of the weights of :func:`route_experts` for the logits [N, E]
+    (their dtype), given dweights fp32 [N, k] and the forward's logits, idx and
+    options. Slots whose index lies outside [0, E) contribute nothing."""
+    dev = _cuda_matrix("logits", logits)
+    n, E = logits.shape
+    _cuda_matrix("idx", idx)
+    k = idx.shape[1]
+    _need("idx", idx, torch.int32, (n, k), dev)
+    _need("dweights", dweights, torch.float32, (n, k), dev)
+    dlogits = torch.empty_like(logits)
+    _call(dev, "agm_route_experts_backward", ptr(dweights), ptr(logits), dtype_code(logits.dtype), n, E, k, ptr(idx),
+          _score_code(score), int(renormalize), float(scale), ptr(dlogits))
+    return dlogits
+
+
+FP8_BLOCK = 128  # elements that share a scale
+
+
+class FP8Tensor(NamedTuple):
+    """A matrix (or stack of weight matrices) in block-scaled e4m3.
+
+    ``q``: torch.float8_e4m3fn, [rows, width] or [G, n, width].
+    ``scales``: uint8 exponents + 127 in tiles of 128 rows x 4 blocks of 128,
+    [ceil(rows / 128), ceil(width / 512), 512] (with a leading G for weights):
+    row r and block b at byte 16 * (r % 32) + 4 * (r % 128 / 32) + b % 4 of
+    tile (r / 128, b / 4). An element stands for q * 2^(byte - 127)."""
+    q: torch.Tensor
+    scales: torch.Tensor
+
+
+def _scale_shape(rows: int, width: int) -> tuple:
+    return ((rows + 127) // 128, (width + 511) // 512, 512)
+
+
+def _need_fp8(what: str, t: FP8Tensor, dim: int, dev: Optional[torch.device] = None) -> torch.device:
+    if not isinstance(t, FP8Tensor):
+        raise _lib.MoEKernelError(f"{what} must be an FP8Tensor, not {type(t).__name__}")
+    dev = _cuda_matrix(f"{what}.q", t.q, dim) if dev is None else dev
+    _need(f"{what}.q", t.q, torch.float8_e4m3fn, t.q.shape, dev)
+    _cuda_matrix(f"{what}.q", t.q, dim)
+    _need(f"{what}.scales", t.scales, torch.uint8, (*t.q.shape[:-2], *_scale_shape(*t.q.shape[-2:])), dev)
+    return dev
+
+
+def quantize_fp8(x: torch.Tensor) -> FP8Tensor:
+    """Rows [rows, width] (width a multiple of 16) -> e4m3 with one power-of-two
+    scale per 128 elements of a row: 2^p, p the least integer with
+    amax <= 448 * 2^p. NaN and infinities become NaN and do not count for amax."""
+    dev = _cuda_matrix("x", x)
+    rows, width = x.shape
+    t = FP8Tensor(torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=dev),
+                  torch.empty(_scale_shape(rows, width), dtype=torch.uint8, device=dev))
+    _call(dev, "agm_quantize_fp8", ptr(x), dtype_code(x.dtype), rows, width, ptr(t.q), ptr(t.scales))
+    return t
+
+
+def quantize_fp8_weight(w: torch.Tensor) -> FP8Tensor:
+    """Weights [G, n, width] (nn.Linear layout) -> e4m3 with one scale per
+    128 x 128 block, chosen as in :func:`quantize_fp8`."""
+    dev = _cuda_matrix("w", w, 3)
+    G, n, width = w.shape
+    t = FP8Tensor(torch.empty(G, n, width, dtype=torch.float8_e4m3fn, device=dev),
+                  torch.empty(G, *_scale_shape(n, width), dtype=torch.uint8, device=dev))
+    _call(dev, "agm_quantize_fp8_weight", ptr(w), dtype_code(w.dtype), G, n, width, ptr(t.q), ptr(t.scales))
+    return t
+
+
+def dequantize_fp8(t: FP8Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values an :class:`FP8Tensor` stands for, rounded once to ``dtype``."""
+    dev = _need_fp8("t", t, t.q.dim() if isinstance(t, FP8Tensor) and t.q.dim() == 3 else 2)
+    rows, width = t.q.shape[-2:]
+    G = t.q.shape[0] if t.q.dim() == 3 else 1
+    out = torch.empty(t.q.shape, dtype=dtype, device=dev)
+    _call(dev, "agm_dequantize_fp8", ptr(t.q), ptr(t.scales), G, rows, width, dtype_code(dtype), ptr(out))
+    return out
+
+
+def grouped_gemm_fp8(a: FP8Tensor, w: FP8Tensor, bias: Optional[torch.Tensor] = None, *, relu: bool = False,
+                     seg_start: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
+                     out_dtype: torch.dtype = torch.bfloat16, mode: int = _lib.AGM_FP8_AUTO,
+                     out: Optional[torch.Tensor] = None, err: Optional[torch.Tensor] = None
+                     ) -> Union[torch.Tensor, FP8Tensor]:
+    """act(a @ w[g]^T + bias[g]) for the rows of every group g, on the 8-bit tensor cores with fp32 sums.
+
+    a: rows [R, K] (:func:`quantize_fp8`); w: [G, N, K]
+    (:func:`quantize_fp8_weight`); bias: fp32 [G, N] or None; K and N multiples
+    of 16, G <= 512. ``seg_start`` int32 [G + 1] and ``counts`` int32 [G]: group
+    g holds the rows [seg_start[g], seg_start[g] + counts[g]); segments start
+    at multiples of 128 and do not overlap. The rows behind a group's last, up
+    to the next multiple of 128, come back as zeros; other rows of the output
+    are not written (``out`` keeps them). Without them G is 1 and every row
+    belongs to the group.
+
+    out_dtype: torch.bfloat16, torch.float16, or torch.float8_e4m3fn for an
+    FP8Tensor quantised from the fp32 results (the next product's input).
+    Segments that do not fit are left out and set the device error word ``err``."""
+    dev = _need_fp8("a", a, 2)
+    _need_fp8("w", w, 3, dev)
+    R, K = a.q.shape
+    G, N, Kw = w.q.shape
+    if Kw != K:
+        raise _lib.MoEKernelError(f"a has {K} features, w expects {Kw}")
+    if bias is not None:
+        _need("bias", bias, torch.float32, (G, N), dev)
+    if (seg_start is None) != (counts is None):
+        raise _lib.MoEKernelError("seg_start and counts go together")
+    if counts is not None:
+        _need("seg_start", seg_start, torch.int32, (G + 1,), dev)
+        _need("counts", counts, torch.int32, (G,), dev)
+    if err is not None:
+        _need("err", err, torch.int32, (1,), dev)
+    scales = None
+    if out_dtype == torch.float8_e4m3fn:
+        # whole tiles are defined: bytes of blocks that do not exist are 0
+        scales = torch.zeros(_scale_shape(R, N), dtype=torch.uint8, device=dev)
+    elif out_dtype not in (torch.bfloat16, torch.float16):
+        raise _lib.MoEKernelError(f"out_dtype must be bfloat16, float16 or float8_e4m3fn, not {out_dtype}")
+    if out is None:
+        out = torch.empty(R, N, dtype=out_dtype, device=dev)
+    else:
+        _need("out", out, out_dtype, (R, N), dev)
+    _call(dev, "agm_grouped_gemm_fp8", ptr(a.q), ptr(a.scales), R, ptr(w.q), ptr(w.scales), ptr(bias), G, N, K,
+          ptr(seg_start), ptr(counts), int(relu), mode, ptr(out), 0 if scales is not None else dtype_code(out_dtype),
+          ptr(scales), ptr(err))
+    return out if scales is None else FP8Tensor(out, scales)
+
+
+def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, w1: FP8Tensor, b1: torch.Tensor,
+                    w2: FP8Tensor, b2: torch.Tensor, *, residual: Optional[torch.Tensor] = None,
+                    workspace: Optional[torch.Tensor] = None, check_errors: bool = False) -> torch.Tensor:
+    """The routed experts of a MoE block with 8-bit weights:
+    out[t] = (residual[t] +) sum_r weights[t, r] * y(t, r), with
+    y(t, r) = W2[e] Q(relu(W1[e] Q(x[t]) + b1[e])) + b2[e], e = idx[t, r], and Q
+    the quantisation of :func:`quantize_fp8`. y has x's dtype, sums are fp32.
+
+    x [N, d] bf16 or fp16; idx int32 [N, k] and weights fp32 [N, k], as
+    :func:`route_experts` returns them (slots outside [0, E) contribute
+    nothing); w1 [E, H, d] and w2 [E, d, H] from :func:`quantize_fp8_weight`;
+    b1 [E, H] and b2 [E, d] fp32; d and H multiples of 16, E <= 512, k <= 32.
+    The workspace (uint8, agm_moe_experts_fp8_workspace_bytes) is allocated per
+    call unless given, so calls on several streams and captured graphs do not
+    share one by accident."""
+    lib = load()
+    dev = _cuda_matrix("x", x)
+    n, d = x.shape
+    _need_fp8("w1", w1, 3, dev)
+    _need_fp8("w2", w2, 3, dev)
+    E, H, dw = w1.q.shape
+    if dw != d or w2.q.shape != (E, d, H):
+        raise _lib.MoEKernelError(f"w1 {tuple(w1.q.shape)} and w2 {tuple(w2.q.shape)} do not fit x {tuple(x.shape)}")
+    _cuda_matrix("idx", idx)
+    k = idx.shape[1]
+    _need("idx", idx, torch.int32, (n, k), dev)
+    _need("weights", weights, torch.float32, (n, k), dev)
+    _need("b1", b1, torch.float32, (E, H), dev)
+    _need("b2", b2, torch.float32, (E, d), dev)
+    if residual is not None:
+        _need("residual", residual, x.dtype, (n, d), dev)
+    if workspace is None:
+        nbytes = int(lib.agm_moe_experts_fp8_workspace_bytes(n, d, E, k, H))
+        workspace = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
+    elif workspace.device != dev or workspace.dtype != torch.uint8:
+        raise _lib.MoEKernelError(f"workspace must be a uint8 tensor on {dev}")
+    out = torch.empty_like(x)
+    _call(dev, "agm_moe_experts_fp8", ptr(x), dtype_code(x.dtype), n, d, E, k, H, ptr(idx), ptr(weights), ptr(w1.q),
+          ptr(w1.scales), ptr(b1), ptr(w2.q), ptr(w2.scales), ptr(b2), ptr(residual), ptr(out), ptr(workspace),
+          workspace.numel())
+    if check_errors:
+        code = _lib.read_device_error(workspace[:4].view(torch.int32))
+        if code:
+            raise _lib.MoEKernelError(f"device error word 0x{code:x} after agm_moe_experts_fp8")
+    return out

@@ -503,6 +503,87 @@ AGM_API int agm_decode_tile_layout(const void* w, void* out, int dtype, int64_t 
  * the word was 0, AGM_ERR_DEVICE otherwise.                                */
 AGM_API int agm_read_device_error(int* err, int* code, void* stream);
 
+/* General expert routing of given router logits (any source, up to 512
+ * experts): a superset of the reference's top-k selection (agillm41.py:4418-4419).
+ *   logits [n, E] (dtype)  -> idx int32 [n, k], weights fp32 [n, k]
+ *   score       AGM_ROUTE_SOFTMAX (over all E) or AGM_ROUTE_SIGMOID
+ *   bias        nullable fp32 [E]: added to the scores for the choice only
+ *   n_groups    E is split into this many equal groups (at most 32); the
+ *               top_groups with the largest sum of their two largest choosable
+ *               keys (scores without a bias) are kept
+ *   renormalize divide the weights by their sum over the k chosen
+ *   scale       factor of the weights
+ * Ties go to the lowest index. An expert whose logit is -inf or whose key is
+ * -inf or NaN is never chosen; a slot without an expert gets index -1 and
+ * weight 0. A row with a NaN logit (or +inf under softmax) gets NaN weights. */
+#define AGM_ROUTE_SOFTMAX 0
+#define AGM_ROUTE_SIGMOID 1
+#define AGM_ROUTE_MAX_EXPERTS 512
+#define AGM_ROUTE_MAX_TOPK 32
+AGM_API int agm_route_experts(const void* logits, int dtype, int64_t n_tokens, int n_experts, int top_k, int score,
+                              const float* bias, int n_groups, int top_groups, int renormalize, float scale,
+                              int32_t* idx, float* weights, void* stream);
+/* Gradient of agm_route_experts' weights: dweights fp32 [n, k], the forward's
+ * logits and idx -> dlogits [n, E] (dtype), written whole. An index outside
+ * [0, E) contributes nothing; a repeated index adds up. */
+AGM_API int agm_route_experts_backward(const float* dweights, const void* logits, int dtype, int64_t n_tokens,
+                                       int n_experts, int top_k, const int32_t* idx, int score, int renormalize,
+                                       float scale, void* dlogits, void* stream);
+
+/* Block-scaled 8-bit floating point. A matrix [rows, width] is e4m3 bytes plus
+ * one power-of-two scale per 128 consecutive elements of a row; weights share
+ * one scale per 128 x 128 block. Scales are E8M0 bytes (exponent + 127) in
+ * 512-byte tiles [ceil(rows / 128)][ceil(width / 512)][512]: row r, block b at
+ * byte 16 * (r % 32) + 4 * (r % 128 / 32) + b % 4 of tile (r / 128, b / 4).
+ * The exponent is the least p with max|x| <= 448 * 2^p (>= -127), values are
+ * rounded to nearest even; NaN and infinities become NaN and do not count for
+ * the maximum. width is a multiple of 16. */
+AGM_API size_t agm_fp8_scale_bytes(int64_t rows, int width);
+AGM_API int agm_quantize_fp8(const void* x, int dtype, int64_t rows, int width, void* q, void* scales, void* stream);
+/* w [groups, n, width] -> q [groups, n, width], scales [groups][tiles of one matrix] */
+AGM_API int agm_quantize_fp8_weight(const void* w, int dtype, int64_t groups, int n, int width, void* q, void* scales,
+                                    void* stream);
+/* q, scales -> out [groups, rows, width] (dtype): q * 2^p, rounded once. */
+AGM_API int agm_dequantize_fp8(const void* q, const void* scales, int64_t groups, int64_t rows, int width, int dtype,
+                               void* out, void* stream);
+
+/* c[r, :] = act(a[r, :] @ w[g]^T + bias[g]) over block-scaled operands on the
+ * tensor cores (fp32 accumulation).
+ *   a [a_rows, k_in] e4m3 + a_scales, w [groups, n_out, k_in] e4m3 + w_scales,
+ *   bias nullable fp32 [groups, n_out]
+ *   seg_start int32 [groups + 1], counts int32 [groups] (device): group g's
+ *     rows are [seg_start[g], seg_start[g] + counts[g]); seg_start are
+ *     multiples of 128 and segments do not overlap. A segment's rows behind
+ *     its count, up to the next multiple of 128, are written as zeros; all
+ *     other rows of c are left as they were. Both null: groups is 1 and the
+ *     group holds all a_rows rows.
+ *   c [a_rows, n_out]: c_dtype AGM_BF16 or AGM_F16; or, with c_scales, e4m3
+ *     quantised from the fp32 results (c_dtype is then ignored)
+ *   mode: AGM_FP8_AUTO, or one of the two kernels for comparisons
+ *   err: device int (nullable)                                             */
+#define AGM_FP8_AUTO 0
+#define AGM_FP8_ROWS 1    /* 256-row tiles on CTA pairs */
+#define AGM_FP8_WEIGHTS 2 /* weights as the MMA's row operand, for few rows per group */
+AGM_API int agm_grouped_gemm_fp8(const void* a, const void* a_scales, int64_t a_rows, const void* w,
+                                 const void* w_scales, const float* bias, int groups, int n_out, int k_in,
+                                 const int32_t* seg_start, const int32_t* counts, int relu, int mode, void* c,
+                                 int c_dtype, void* c_scales, int* err, void* stream);
+
+/* The routed experts of a MoE block with 8-bit weights, given the routing:
+ *   out[t] = (residual[t] +) sum_r weights[t, r] * y(t, r),
+ *   y(t, r) = W2[e] Q(relu(W1[e] Q(x[t]) + b1[e])) + b2[e],  e = idx[t, r]
+ * with Q the quantisation above; y is rounded to dtype, sums are fp32. Slots
+ * whose index is outside [0, E) contribute nothing.
+ *   x, residual (nullable), out [n, d]: AGM_BF16 or AGM_F16
+ *   w1 [E, hidden, d], w2 [E, d, hidden] e4m3 with their scales, b1 [E, hidden], b2 [E, d] fp32
+ * The workspace's first int is the device error word (cleared by the call). */
+AGM_API size_t agm_moe_experts_fp8_workspace_bytes(int64_t n_tokens, int d, int n_experts, int top_k, int hidden);
+AGM_API int agm_moe_experts_fp8(const void* x, int dtype, int64_t n_tokens, int d, int n_experts, int top_k, int hidden,
+                                const int32_t* idx, const float* weights, const void* w1, const void* s1,
+                                const float* b1, const void* w2, const void* s2, const float* b2,
+                                const void* residual, void* out, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
 #ifdef __cplusplus
 }
 #endif
