@@ -68,6 +68,49 @@ __device__ __forceinline__ float2 unpack_e4m3x2(uint32_t v) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));  // every e4m3 value is a half
 }
 
+// Packed fp32 pairs (one instruction for two adds or products).
+__device__ __forceinline__ void add2(uint32_t& x, uint32_t& y, float a, float b) {
+  asm("{\n\t.reg .b64 v, w;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 w, {%2, %3};\n\tadd.rn.f32x2 v, v, w;\n\t"
+      "mov.b64 {%0, %1}, v;\n\t}"
+      : "+r"(x), "+r"(y)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void scale2(uint32_t& x, uint32_t& y, float s) {
+  asm("{\n\t.reg .b64 v, w;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 w, {%2, %2};\n\tmul.rn.f32x2 v, v, w;\n\t"
+      "mov.b64 {%0, %1}, v;\n\t}"
+      : "+r"(x), "+r"(y)
+      : "f"(s));
+}
+// max(v, 0) that keeps NaN.
+__device__ __forceinline__ float relu_keep_nan(float v) {
+  float o;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(o) : "f"(v));
+  return o;
+}
+
+// One lane of the converged warp. The compiler issues tcgen05 and TMA
+// instructions behind it once; behind `lane == 0` it loops over the active
+// lanes around every one of them, which held the MMA issue to 2.06 PFLOP/s
+// where it now reaches 2.47 (rows kernel, 75,776 x 3200 by 1280 x 3200).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(p)
+      :
+      : "memory");
+  return p != 0;
+}
+
+// Arrive on an mbarrier of another CTA of the cluster (cluster address). It
+// orders this CTA's work only: a release at cluster scope also waits for the
+// thread's outstanding global stores, over a microsecond in an epilogue.
+__device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // ---------------------------------------------------------------------------
 // tcgen05 with block scales
 // ---------------------------------------------------------------------------

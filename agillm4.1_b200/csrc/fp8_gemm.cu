@@ -162,8 +162,6 @@ __device__ __forceinline__ Unit weights_unit(const Groups& s, int groups, int t,
   return u;
 }
 
-__device__ __forceinline__ float relu_keep_nan(float v) { return v < 0.f ? 0.f : v; }
-
 // OUT: __nv_bfloat16, __half, or __nv_fp8_e4m3 (block-scaled output).
 template <typename OUT, bool RELU>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -251,7 +249,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           ok = false;
           break;
         }
-        if (lane == 0) {
+        if (elect_one()) {
           const bool sf = (kb & 3) == 0;
           if (leader) mbar_arrive_expect_tx(&full[stage], 2 * (kPA + kPB + (sf ? kPSf : 0)));
           const uint32_t fb = full0 + stage * 8;
@@ -315,7 +313,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             sfb = sfa + 4;
           }
           tc_fence_after();
-          if (lane == 0) {
+          if (elect_one()) {
             if ((kb & 3) == 0) {
               const uint32_t src = sSf_addr + stage * kPSf;
               tmem_copy_scales<2>(sfa, smem_desc_scale(src));
@@ -339,7 +337,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (lane == 0) umma_commit_pair(drain, 0x1);
+      if (elect_one()) umma_commit_pair(drain, 0x1);
       __syncwarp();
       mbar_wait(drain, 0, args.err, kErrTimeoutDrain);
     }
@@ -370,48 +368,76 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       tc_fence_after();
       uint32_t r[128];
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kAccStep + half * 128;
+      // The common columns are the last 32 of accumulator 0 and the first 32
+      // of accumulator 1: they are read and released before the others.
+      if (half != acc) {
+        if (work) {
+          if (acc)
+            tmem_ld_32x32b_x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+          else
+            tmem_ld_32x32b_x32(taddr + 96, *reinterpret_cast<uint32_t(*)[32]>(&r[96]));
+          tmem_ld_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (leader)
+            mbar_arrive(shared_cols);
+          else
+            mbar_arrive_peer(shared0);
+        }
+      }
       if (work) {
-        const uint32_t taddr =
-            tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kAccStep + half * 128;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld_32x32b_x32(taddr + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(&r[32 * q]));
+        if (half == acc || !acc) tmem_ld_32x32b_x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+        tmem_ld_32x32b_x32(taddr + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+        tmem_ld_32x32b_x32(taddr + 64, *reinterpret_cast<uint32_t(*)[32]>(&r[64]));
+        if (half == acc || acc) tmem_ld_32x32b_x32(taddr + 96, *reinterpret_cast<uint32_t(*)[32]>(&r[96]));
         tmem_ld_wait();
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        // The common columns are the last 32 of accumulator 0 and the first 32 of accumulator 1.
-        if (half != acc) {
-          if (leader)
-            mbar_arrive(shared_cols);
-          else
-            mbar_arrive_remote(shared0);
-        }
         if (leader)
           mbar_arrive(&acc_empty[acc]);
         else
-          mbar_arrive_remote(acc_empty0 + acc * 8);
+          mbar_arrive_peer(acc_empty0 + acc * 8);
       }
       if (!work) continue;
-      const bool live = lane < r_valid;
+      const bool whole = r_valid >= 32 && n_valid >= 128;
       const float* brow = args.bias ? args.bias + static_cast<int64_t>(u.g) * args.n + n0 : nullptr;
+      if (brow) {
 #pragma unroll
-      for (int q = 0; q < 32; ++q) {
-        float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-        const bool in = 4 * q < n_valid;
-        if (brow && in) b = __ldg(reinterpret_cast<const float4*>(brow + 4 * q));
-        const float bv[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float v = __uint_as_float(r[4 * q + j]) + bv[j];
-          if (RELU) v = relu_keep_nan(v);
-          r[4 * q + j] = __float_as_uint(live && in ? v : 0.f);
+        for (int q = 0; q < 32; ++q) {
+          if (whole || 4 * q < n_valid) {
+            const float4 b = __ldg(reinterpret_cast<const float4*>(brow + 4 * q));
+            add2(r[4 * q], r[4 * q + 1], b.x, b.y);
+            add2(r[4 * q + 2], r[4 * q + 3], b.z, b.w);
+          }
         }
       }
-      if constexpr (OUT8) {
-        float m = 0.f;
+      if (RELU) {
 #pragma unroll
-        for (int j = 0; j < 128; ++j) m = fmaxf(m, finite_abs(__uint_as_float(r[j])));
+        for (int j = 0; j < 128; ++j) r[j] = __float_as_uint(relu_keep_nan(__uint_as_float(r[j])));
+      }
+      if (!whole) {
+        const bool live = lane < r_valid;
+#pragma unroll
+        for (int j = 0; j < 128; ++j) r[j] = live && j < n_valid ? r[j] : 0u;
+      }
+      if constexpr (OUT8) {
+        float mx[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], fabsf(__uint_as_float(r[j])));  // passes over NaN
+        float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if (m == __uint_as_float(0x7f800000u)) {
+          m = 0.f;
+#pragma unroll
+          for (int j = 0; j < 128; ++j) {
+            m = fmaxf(m, finite_abs(__uint_as_float(r[j])));
+            r[j] = __float_as_uint(inf_to_nan(__uint_as_float(r[j])));
+          }
+        }
         const uint32_t byte = scale_byte(m);
         const float inv = inv_scale(byte);
         if (lane == 0) bulk_wait_group_read0();
@@ -422,8 +448,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int j = 16 * q + 4 * i;
-            w[i] = pack_e4m3x4(inf_to_nan(__uint_as_float(r[j])) * inv, inf_to_nan(__uint_as_float(r[j + 1])) * inv,
-                               inf_to_nan(__uint_as_float(r[j + 2])) * inv, inf_to_nan(__uint_as_float(r[j + 3])) * inv);
+            scale2(r[j], r[j + 1], inv);
+            scale2(r[j + 2], r[j + 3], inv);
+            w[i] = pack_e4m3x4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]),
+                               __uint_as_float(r[j + 3]));
           }
           *reinterpret_cast<uint4*>(stg + lane * 128 + ((q ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -566,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = false;
           break;
         }
-        if (lane == 0) {
+        if (elect_one()) {
           const bool sf = (kb & 3) == 0;
           mbar_arrive_expect_tx(&full[stage], Cfg::kW + boxes * 32 * kBK + (sf ? Cfg::kSf : 0));
           tma_load_3d(sW + stage * Cfg::kW, &tmW, kb * kBK, u.nb * 128, u.g, &full[stage]);
@@ -636,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         tc_fence_after();
-        if (lane == 0) {
+        if (elect_one()) {
           if ((kb & 3) == 0) {
             const uint32_t src = sSf_addr + stage * Cfg::kSf;
             const uint32_t dst = tmem_base + Cfg::kSfCol + slot * 8;
@@ -660,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if (lane == 0) umma_commit(drain);
+    if (elect_one()) umma_commit(drain);
     __syncwarp();
     mbar_wait(drain, 0, args.err, kErrTimeoutDrain);
   } else {
