@@ -19,10 +19,26 @@
 // how an exponential is rounded. Equal logits with equal biases are equal
 // keys and need no second look.
 //
-// Mapping: L lanes hold a token's E logits in registers, V each (lane i holds
-// experts i, i + L, ...). Few experts take few lanes, so a warp routes 8
-// tokens of a 16-expert block; grouped routing takes the whole warp.
+// Two forward kernels:
+//
+// * route_kernel, any E <= 512, k <= 32 and grouping: L lanes hold a token's
+//   logits, V each (lane i holds experts i, i + L, ...) and pick k times the
+//   largest key. Few experts take few lanes, so a warp routes 8 tokens of a
+//   16-expert block; grouped routing takes the whole warp.
+//
+// * route_wide_kernel, E >= 32 and k <= 8, bound by its instructions rather
+//   than by memory if it picked that way (65,536 x 256 grouped top-8 took 232
+//   us). Lane c of L holds the experts [c * per, (c + 1) * per), a whole group
+//   or a whole part of one, so a group's two largest keys are found without
+//   talking to other lanes. The k-th largest of the maxima of 4 L sub-blocks
+//   bounds the k-th largest key from below; the few keys that reach it (9 to
+//   12 for k = 8) go to a list in index order, where each finds its rank by
+//   counting. Where keys are too close to be told apart, those of the list,
+//   or the two that make a group's score, are formed again in fp64. Only rows
+//   with NaN, +inf under softmax, or more than 32 keys at the border go to
+//   the other kernel's selection, one by one.
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "common.cuh"
@@ -275,6 +291,414 @@ __global__ void __launch_bounds__(kRouteThreads)
   }
 }
 
+// The exact selection of one token by a whole warp; slot r in lane r.
+template <typename T>
+__device__ __noinline__ int select_exactly(const T* __restrict__ row, const RouteArgs& a) {
+  constexpr int V = AGM_ROUTE_MAX_EXPERTS / 32;
+  const int lane = lane_id();
+  float l[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) l[j] = lane + 32 * j < a.n_experts ? Traits<T>::to_f(row[lane + 32 * j]) : kNegInf;
+  int sel[1];
+  select_experts<double, 32, V, 1>(l, a, lane, sel);
+  return sel[0];
+}
+
+// Approximate exponential (within 2^-22, relative, and 1.5 |v| 2^-24 for its
+// rounded argument) and reciprocal (2^-23). A sigmoid 1 / (1 + e^-l) formed
+// from them is off by at most s (1 - s) times the exponential's error, which
+// is below 1.4 * 2^-24, plus s * 3 * 2^-24: two keys by 10 * 2^-24 (1 + |c|)
+// together with the bias' add, two sums of two by twice that. A softmax score
+// s is off by at most 30 s 2^-24 (the sum's terms and tree for E <= 512), and
+// all scores sum to 1, so two keys, or two sums of two, by
+// 32 * 2^-24 (1 + |c|).
+__device__ __forceinline__ float fast_exp(float v) {
+  float o;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(o) : "f"(v * 1.4426950408889634f));
+  return o;
+}
+__device__ __forceinline__ float fast_rcp(float v) {
+  float o;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(o) : "f"(v));
+  return o;
+}
+
+__device__ __forceinline__ void order2(float& a, float& b) {  // a >= b
+  const float t = fminf(a, b);
+  a = fmaxf(a, b);
+  b = t;
+}
+__device__ __forceinline__ void bitonic8(float (&v)[8]) {  // a bitonic sequence, to descending order
+#pragma unroll
+  for (int d = 4; d; d >>= 1)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (!(i & d)) order2(v[i], v[i + d]);
+}
+
+// e / per for e < 512 (the quotient is at least 1 / 64 away from the next integer).
+__device__ __forceinline__ int owner(int e, float inv_per) { return static_cast<int>((e + 0.5f) * inv_per); }
+
+// Score in fp64; m and t: the softmax's maximum and sum.
+__device__ __noinline__ double exact_score(float l, bool sigmoid, float m, double t) {
+  const double z = exp(sigmoid ? -static_cast<double>(l) : static_cast<double>(l) - m);
+  return sigmoid ? 1.0 / (1.0 + z) : z / t;
+}
+
+constexpr int kWideTopK = 8;
+constexpr int kWideList = 32;
+
+template <int L, int V>
+struct WideSmem {
+  static constexpr int kTok = 32 / L;
+  static constexpr int kLane = V + 4;  // floats between two lanes' experts: 16-byte rows, no bank conflicts
+  float logit[kTok][L * kLane];
+  float key[kTok][kWideList];
+  double exact[kTok][kWideList];
+  int id[kTok][kWideList];
+  int sel[kTok][kWideTopK];
+};
+
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    return __ldcs(reinterpret_cast<const float4*>(p));
+  } else {
+    const uint2 u = __ldcs(reinterpret_cast<const uint2*>(p));
+    const T* h = reinterpret_cast<const T*>(&u);
+    return make_float4(Traits<T>::to_f(h[0]), Traits<T>::to_f(h[1]), Traits<T>::to_f(h[2]), Traits<T>::to_f(h[3]));
+  }
+}
+
+// max that keeps NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float o;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(o) : "f"(a), "f"(b));
+  return o;
+}
+// bits |= v >= bound ? bit : 0
+__device__ __forceinline__ void mark_if_ge(uint32_t& bits, float v, float bound, uint32_t bit) {
+  asm("{\n\t.reg .pred p;\n\tsetp.ge.f32 p, %1, %2;\n\t@p or.b32 %0, %0, %3;\n\t}"
+      : "+r"(bits)
+      : "f"(v), "f"(bound), "r"(bit));
+}
+
+// RAW: neither bias nor groups, the key is the logit. Otherwise the register
+// key is the approximate score (plus bias); the list holds exact logits where
+// there is no bias.
+template <typename T, int L, int V, bool RAW>
+__global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
+    route_wide_kernel(const T* __restrict__ logits, RouteArgs a, int per, int run, int32_t* __restrict__ idx,
+                      float* __restrict__ weights) {
+  using Smem = WideSmem<L, V>;
+  constexpr int TOK = Smem::kTok, LD = Smem::kLane, SB = V / 4;
+  constexpr uint32_t kAll = 0xffffffffu;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  Smem& sm = reinterpret_cast<Smem*>(smem_raw)[warp_id()];
+  float* bias_s = reinterpret_cast<float*>(smem_raw + sizeof(Smem) * (kRouteThreads / 32));  // [L * LD]
+  const int lane = lane_id(), sub = lane & (L - 1), tok = lane / L;
+  const int E = a.n_experts;
+  const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (kRouteThreads / 32) + warp_id()) * TOK;
+  const int toks = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(TOK), a.n - t0)));
+  const bool grouped = !RAW && a.top_groups < a.n_groups;
+  const bool biased = !RAW && a.bias != nullptr;
+  const bool sigmoid = a.score == AGM_ROUTE_SIGMOID;
+  const float inv_per = 1.f / per;
+  pdl_wait();
+  pdl_trigger();
+  // 1. The tokens' logits to shared memory, as fp32 in the lanes' order;
+  // places of no expert hold -inf.
+  const T* src = logits + t0 * E;
+  if (run) {  // E == L * V, aligned rows: the tokens are one run of 16-byte (8-byte) units
+    constexpr int N = TOK * L * V / 128;
+    float4 f[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      const int i = 128 * q + 4 * lane;
+      f[q] = i / (L * V) < toks ? load4<T>(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if (biased)
+      for (int e = threadIdx.x; e < E; e += kRouteThreads) bias_s[e / V * LD + e % V] = a.bias[e];
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      const int i = 128 * q + 4 * lane, c = i / V;  // c counts lanes over all tokens
+      *reinterpret_cast<float4*>(&sm.logit[0][c * LD + (i - c * V)]) = f[q];
+    }
+  } else {
+    for (int i = lane; i < TOK * L * LD; i += 32) sm.logit[0][i] = kNegInf;
+    __syncwarp();
+    for (int k = 0; k < toks; ++k)
+      for (int e = lane; e < E; e += 32) {
+        const int c = owner(e, inv_per);
+        sm.logit[k][c * LD + (e - c * per)] = Traits<T>::to_f(src[k * E + e]);
+      }
+    if (biased)
+      for (int e = threadIdx.x; e < E; e += kRouteThreads) {
+        const int c = owner(e, inv_per);
+        bias_s[c * LD + (e - c * per)] = a.bias[e];
+      }
+  }
+  __syncthreads();
+  if (toks == 0) return;  // whole warps; no barrier of the CTA follows
+  const uint32_t part = L == 32 ? kAll : ((1u << (L & 31)) - 1u) << (tok * L);
+  const float* my_logit = &sm.logit[tok][sub * LD];
+  // 2. Keys, and per quarter of the lane's experts the two largest.
+  float key[V], m = 0.f, inv_t = 0.f;
+#pragma unroll
+  for (int q = 0; q < V / 4; ++q) {
+    const float4 f = *reinterpret_cast<const float4*>(my_logit + 4 * q);
+    key[4 * q] = f.x, key[4 * q + 1] = f.y, key[4 * q + 2] = f.z, key[4 * q + 3] = f.w;
+  }
+  bool bad = false;
+  if (!sigmoid && !(RAW && a.renormalize)) {
+    m = kNegInf;
+#pragma unroll
+    for (int j = 0; j < V; ++j) m = fmaxf(m, key[j]);
+    m = lanes_max<float, L>(m);
+    bad = m == INFINITY;
+    if (m == kNegInf) m = 0.f;  // exp(-inf - 0) = 0
+    float t = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) t += fast_exp(key[j] - m);
+    t = lanes_sum<float, L>(t);
+    inv_t = t > 0.f ? 1.f / t : 0.f;
+  }
+  float top[8], g1 = kNegInf, g2 = kNegInf;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    float k1 = kNegInf, k2 = kNegInf;
+    if constexpr (!RAW) {
+      float s[SB];
+      if (sigmoid) {
+#pragma unroll
+        for (int j = 0; j < SB; ++j) s[j] = fast_rcp(1.f + fast_exp(-key[b * SB + j]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < SB; ++j) s[j] = fast_exp(key[b * SB + j] - m) * inv_t;
+      }
+      if (biased) {
+#pragma unroll
+        for (int j = 0; j < SB; ++j) s[j] += bias_s[sub * LD + b * SB + j];
+      }
+#pragma unroll
+      for (int j = 0; j < SB; ++j) {
+        const float c = key[b * SB + j] == kNegInf ? kNegInf : s[j];
+        k2 = fmaxf(k2, fminf(k1, c));
+        k1 = max_nan(k1, c);
+        key[b * SB + j] = c;
+      }
+      g2 = fmaxf(fmaxf(g2, k2), fminf(g1, k1));
+      g1 = fmaxf(g1, k1);
+    } else {
+#pragma unroll
+      for (int j = 0; j < SB; ++j) k1 = max_nan(k1, key[b * SB + j]);
+    }
+    bad |= k1 != k1;
+    top[b] = k1;
+  }
+  bool near = false, kept = true;
+  double exact_t = 1.0;
+  bool have_t = sigmoid;
+  // The softmax's sum in fp64, formed when first needed (whole warps).
+  auto need_sum = [&]() {
+    if (have_t) return;
+    have_t = true;
+    double t = 0.0;
+    for (int j = 0; j < V; ++j) t += exact_score(my_logit[j], false, m, 1.0);
+    exact_t = lanes_sum<double, L>(t);
+  };
+  if (grouped) {
+    const int span = L / a.n_groups;  // lanes of a group
+    const float lane2 = g2;           // the lane's own second key
+    for (int o = 1; o < span; o <<= 1) {
+      const float o1 = __shfl_xor_sync(kAll, g1, o), o2 = __shfl_xor_sync(kAll, g2, o);
+      g2 = fmaxf(fminf(g1, o1), fmaxf(g2, o2));
+      g1 = fmaxf(g1, o1);
+    }
+    const float score = g2 > kNegInf ? g1 + g2 : g1;
+    const float close = (sigmoid ? 20.f : 32.f) * 0x1p-24f * (1.f + fabsf(score));
+    int rank = 0;
+    for (int o = span; o < L; o += span) {
+      const float so = __shfl_sync(kAll, score, (lane & ~(L - 1)) | ((sub + o) & (L - 1)));
+      rank += so > score;
+      near |= fabsf(so - score) <= close;
+    }
+    if (__any_sync(kAll, near)) {
+      // The group scores again, from the exact keys of the one or two (more
+      // only where they are close) largest in every lane.
+      need_sum();
+      const float cut = lane2 - (sigmoid ? 20.f : 64.f) * 0x1p-24f * (1.f + fabsf(lane2));
+      uint32_t pair = 0;
+#pragma unroll
+      for (int j = 0; j < V; ++j) mark_if_ge(pair, key[j], lane2 > kNegInf ? cut : -FLT_MAX, 1u << j);
+      double e1 = -INFINITY, e2 = -INFINITY;
+      while (pair) {
+        const int j = __ffs(pair) - 1;
+        pair &= pair - 1;
+        const double d = exact_score(my_logit[j], sigmoid, m, exact_t) + (biased ? bias_s[sub * LD + j] : 0.f);
+        e2 = fmax(e2, fmin(e1, d));
+        e1 = fmax(e1, d);
+      }
+      for (int o = 1; o < span; o <<= 1) {
+        const double o1 = __shfl_xor_sync(kAll, e1, o), o2 = __shfl_xor_sync(kAll, e2, o);
+        e2 = fmax(fmin(e1, o1), fmax(e2, o2));
+        e1 = fmax(e1, o1);
+      }
+      const double exact = e2 > -INFINITY ? e1 + e2 : e1;
+      rank = 0;
+      for (int o = span; o < L; o += span) {
+        const int other = (sub + o) & (L - 1);
+        const double so = __shfl_sync(kAll, exact, (lane & ~(L - 1)) | other);
+        rank += so > exact || (so == exact && other < sub);
+      }
+      near = false;
+    }
+    kept = rank < a.top_groups;
+    if (!kept)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) top[b] = kNegInf;
+  }
+  // 3. A bound that at least k keys reach: the k-th largest quarter maximum.
+  order2(top[0], top[1]);
+  order2(top[2], top[3]);
+  order2(top[0], top[2]);
+  order2(top[1], top[3]);
+  order2(top[1], top[2]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top[7 - i] = __shfl_xor_sync(kAll, top[i], 1);
+  bitonic8(top);
+#pragma unroll
+  for (int o = 2; o < L; o <<= 1) {
+    float other[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) other[i] = __shfl_xor_sync(kAll, top[i], o);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top[i] = fmaxf(top[i], other[7 - i]);
+    bitonic8(top);
+  }
+  float bound = top[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) bound = i < a.k ? top[i] : bound;
+  const float error = (sigmoid ? 10.f : 32.f) * 0x1p-24f;  // of (1 + |key|)
+  if (!RAW) bound -= 2.f * error * (1.f + fabsf(bound));
+  if (!(bound > kNegInf)) bound = -FLT_MAX;
+  // 4. The keys that reach it, in index order.
+  uint32_t hit = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) mark_if_ge(hit, key[j], bound, 1u << j);
+  if (!kept) hit = 0;
+  const int count = __popc(hit);
+  int upto = count;
+#pragma unroll
+  for (int o = 1; o < L; o <<= 1) {
+    const int u = __shfl_up_sync(kAll, upto, o, L);
+    if (sub >= o) upto += u;
+  }
+  const int total = __shfl_sync(kAll, upto, (lane & ~(L - 1)) | (L - 1));
+  bad = (__ballot_sync(kAll, bad) & part) != 0;
+  bool slow = bad || total > kWideList;
+  for (int at = upto - count; hit && at < kWideList; ++at) {
+    const int j = __ffs(hit) - 1;
+    hit &= hit - 1;
+    float v = my_logit[j];
+    if (biased) {
+      v = sigmoid ? fast_rcp(1.f + fast_exp(-v)) : fast_exp(v - m) * inv_t;  // as in 2
+      v += bias_s[sub * LD + j];
+    }
+    sm.id[tok][at] = sub * per + j;
+    sm.key[tok][at] = v + 0.f;  // -0 = 0
+  }
+  const int len = min(total, kWideList);
+  const int len4 = (len + 3) & ~3;
+  if (sub < len4 - len) sm.key[tok][len + sub] = kNegInf;
+  if (sub < kWideTopK) sm.sel[tok][sub] = -1;
+  __syncwarp();
+  // 5. Each finds its rank: the keys above it. Another key as close as the
+  // error of keys leaves the order open; an equal one goes by its index.
+  const float slack = biased ? error : 0.f;
+  for (int p = sub; p < len; p += L) {
+    const float c = sm.key[tok][p];
+    const float close = slack * (1.f + fabsf(c));
+    const float hi = c + close, lo = c - close;
+    int above = 0, reach = 0;
+    for (int q = 0; q < len4; q += 4) {
+      const float4 o = *reinterpret_cast<const float4*>(&sm.key[tok][q]);
+      above += (o.x > hi) + (o.y > hi) + (o.z > hi) + (o.w > hi);
+      reach += (o.x >= lo) + (o.y >= lo) + (o.z >= lo) + (o.w >= lo);
+    }
+    if (reach != above + 1) {
+      const int ep = sm.id[tok][p], cp = owner(ep, inv_per), ap = cp * LD + ep - cp * per;
+      above = 0;
+      for (int q = 0; q < len; ++q) {
+        const float o = sm.key[tok][q];
+        above += o > c || (o == c && q < p);
+        if (biased && q != p && fabsf(o - c) <= close) {
+          // Equal logits with equal biases are equal keys.
+          const int eq = sm.id[tok][q], cq = owner(eq, inv_per), aq = cq * LD + eq - cq * per;
+          near |= !(bias_s[ap] == bias_s[aq] && sm.logit[tok][ap] == sm.logit[tok][aq]);
+        }
+      }
+    }
+    if (above < a.k) sm.sel[tok][above] = sm.id[tok][p];
+  }
+  if (__any_sync(kAll, near)) {
+    need_sum();
+    near = (__ballot_sync(kAll, near) & part) != 0;
+    if (near)
+      for (int p = sub; p < len; p += L) {
+        const int ep = sm.id[tok][p], cp = owner(ep, inv_per), ap = cp * LD + ep - cp * per;
+        sm.exact[tok][p] = exact_score(sm.logit[tok][ap], sigmoid, m, exact_t) + bias_s[ap];
+      }
+    __syncwarp();
+    if (near)
+      for (int p = sub; p < len; p += L) {
+        const double c = sm.exact[tok][p];
+        int above = 0;
+        for (int q = 0; q < len; ++q) above += sm.exact[tok][q] > c || (sm.exact[tok][q] == c && q < p);
+        if (above < a.k) sm.sel[tok][above] = sm.id[tok][p];
+      }
+  }
+  const bool live = tok < toks;
+  slow = slow && live;
+  __syncwarp();
+  uint32_t open = __ballot_sync(kAll, slow && sub == 0);
+  while (open) {  // tokens left to the exact selection, one at a time
+    const int k = (__ffs(open) - 1) / L;
+    open &= open - 1;
+    const int e = select_exactly<T>(logits + (t0 + k) * E, a);
+    if (lane < a.k) sm.sel[k][lane] = e;
+    __syncwarp();
+  }
+  // 6. Weights.
+  const bool slot = live && sub < a.k;
+  const int e = slot ? sm.sel[tok][sub] : -1;
+  const int c = e >= 0 ? owner(e, inv_per) : 0;
+  const float l = e >= 0 ? sm.logit[tok][c * LD + (e - c * per)] : kNegInf;
+  float p = 0.f, total_p = 1.f;
+  if (a.renormalize) {
+    const float own = sigmoid ? fminf(l, 0.f) : l;
+    const float mx = lanes_max<float, L>(own);
+    if (e >= 0) p = expf(own - mx) / (sigmoid ? 1.f + expf(-fabsf(l)) : 1.f);
+    total_p = lanes_sum<float, L>(p);
+    // A renormalised softmax does not look at the other logits: +inf among them is met here.
+    bad |= !sigmoid && mx == INFINITY;
+  } else if (e >= 0) {
+    p = sigmoid ? expf(fminf(l, 0.f)) / (1.f + expf(-fabsf(l))) : expf(l - m) * inv_t;
+  }
+  if (slot) {
+    bool nan_row = false;
+    if (bad) {  // a NaN bias is no NaN logit
+      for (int i = 0; i < E; ++i) {
+        const int ci = owner(i, inv_per);
+        const float v = sm.logit[tok][ci * LD + (i - ci * per)];
+        nan_row |= v != v || (!sigmoid && v == INFINITY);
+      }
+    }
+    idx[(t0 + tok) * a.k + sub] = e;
+    weights[(t0 + tok) * a.k + sub] = nan_row ? NAN : (e >= 0 ? a.scale * (p / total_p) : 0.f);
+  }
+}
+
 // d l from d w. With s the scores and w' the renormalised weights:
 //   softmax, renormalised   dl_r = scale w'_r (dw_r - sum_j dw_j w'_j)
 //   sigmoid, renormalised   dl_r = scale w'_r (1 - s_r) (dw_r - sum_j dw_j w'_j)
@@ -282,11 +706,58 @@ __global__ void __launch_bounds__(kRouteThreads)
 //   softmax                 dl_e = s_e (scale dw_e - scale sum_j dw_j s_j), every e
 // All but the last are zero outside the chosen experts. An index outside
 // [0, E) is an empty slot; a repeated one adds up.
+// Lane i of L holds the experts [i V, (i + 1) V), so that whole rows move in
+// 16-byte (8-byte) units where they are aligned.
+template <typename T, int V>
+__device__ __forceinline__ void load_span(const T* __restrict__ row, int e0, int E, int vec, float (&l)[V]) {
+  if (vec) {
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+      float v[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+      if (e0 + 4 * q < E) {
+        if constexpr (sizeof(T) == 4) {
+          const float4 f = *reinterpret_cast<const float4*>(row + e0 + 4 * q);
+          v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(row + e0 + 4 * q);
+          const T* h = reinterpret_cast<const T*>(&u);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = Traits<T>::to_f(h[j]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) l[4 * q + j] = v[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) l[j] = e0 + j < E ? Traits<T>::to_f(row[e0 + j]) : kNegInf;
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_span(T* __restrict__ row, int e0, int E, int vec, const float (&v)[V]) {
+  if (vec) {
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+      if (e0 + 4 * q < E) {
+        if constexpr (sizeof(T) == 4)
+          *reinterpret_cast<float4*>(row + e0 + 4 * q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        else
+          *reinterpret_cast<uint2*>(row + e0 + 4 * q) =
+              make_uint2(pack2<T>(v[4 * q], v[4 * q + 1]), pack2<T>(v[4 * q + 2], v[4 * q + 3]));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (e0 + j < E) row[e0 + j] = Traits<T>::from_f(v[j]);
+  }
+}
+
 template <typename T, int L, int V>
 __global__ void __launch_bounds__(kRouteThreads)
     route_backward_kernel(const float* __restrict__ dw, const T* __restrict__ logits, const int32_t* __restrict__ idx,
-                          RouteArgs a, T* __restrict__ dl) {
-  constexpr int KS = L == 32 ? 1 : AGM_ROUTE_MAX_TOPK / 8;
+                          RouteArgs a, int vec, T* __restrict__ dl) {
+  constexpr int KS = AGM_ROUTE_MAX_TOPK / L;
   constexpr int TOK = 32 / L;
   pdl_wait();
   pdl_trigger();
@@ -301,12 +772,9 @@ __global__ void __launch_bounds__(kRouteThreads)
     const T* row = logits + tt * a.n_experts;
     float l[V], m = kNegInf, total = 0.f;
     if (dense) {
+      load_span<T, V>(row, sub * V, a.n_experts, vec, l);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int e = sub + L * j;
-        l[j] = e < a.n_experts ? Traits<T>::to_f(row[e]) : kNegInf;
-        m = fmaxf(m, l[j]);
-      }
+      for (int j = 0; j < V; ++j) m = fmaxf(m, l[j]);
       m = lanes_max<float, L>(m);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -315,33 +783,44 @@ __global__ void __launch_bounds__(kRouteThreads)
       }
       total = lanes_sum<float, L>(total);
     }
+    const float inv_total = total > 0.f ? 1.f / total : total;  // 0 for a row of -inf; NaN stays
     int id[KS];
     float c[KS], g[KS], p[KS], mc = kNegInf;
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
       const int r = sub + L * i;
-      id[i] = r < a.k ? idx[tt * a.k + r] : -1;
-      if (id[i] >= a.n_experts) id[i] = -1;
-      c[i] = id[i] >= 0 ? Traits<T>::to_f(row[id[i]]) : kNegInf;
-      g[i] = id[i] >= 0 ? a.scale * dw[tt * a.k + r] : 0.f;
-      mc = fmaxf(mc, sigmoid ? fminf(c[i], 0.f) : c[i]);
+      id[i] = -1;
+      c[i] = kNegInf;
+      g[i] = p[i] = 0.f;
+      if (L * i < a.k) {
+        id[i] = r < a.k ? idx[tt * a.k + r] : -1;
+        if (id[i] >= a.n_experts) id[i] = -1;
+        if (id[i] >= 0) {
+          c[i] = Traits<T>::to_f(row[id[i]]);
+          g[i] = a.scale * dw[tt * a.k + r];
+        }
+        mc = fmaxf(mc, sigmoid ? fminf(c[i], 0.f) : c[i]);
+      }
     }
-    mc = lanes_max<float, L>(mc);
+    if (a.renormalize) mc = lanes_max<float, L>(mc);
     float sum = 0.f, inner = 0.f;
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
-      if (dense)
-        p[i] = c[i] != kNegInf ? expf(c[i] - m) / total : 0.f;
-      else if (sigmoid)
-        p[i] = c[i] != kNegInf ? expf(fminf(c[i], 0.f) - (a.renormalize ? mc : 0.f)) / (1.f + expf(-fabsf(c[i]))) : 0.f;
-      else
-        p[i] = c[i] != kNegInf ? expf(c[i] - mc) : 0.f;
-      sum += p[i];
+      if (L * i < a.k && id[i] >= 0 && c[i] != kNegInf) {
+        if (dense)
+          p[i] = expf(c[i] - m) * inv_total;
+        else if (sigmoid)
+          p[i] = expf(fminf(c[i], 0.f) - (a.renormalize ? mc : 0.f)) / (1.f + expf(-fabsf(c[i])));
+        else
+          p[i] = expf(c[i] - mc);
+        sum += p[i];
+      }
     }
     if (a.renormalize) {
       sum = lanes_sum<float, L>(sum);
+      const float inv_sum = sum != 0.f ? 1.f / sum : 0.f;
 #pragma unroll
-      for (int i = 0; i < KS; ++i) p[i] = id[i] >= 0 && sum != 0.f ? p[i] / sum : 0.f;
+      for (int i = 0; i < KS; ++i) p[i] *= inv_sum;
     }
     if (a.renormalize || dense) {
 #pragma unroll
@@ -349,20 +828,23 @@ __global__ void __launch_bounds__(kRouteThreads)
       inner = lanes_sum<float, L>(inner);
     }
     float out[V];
+    const float spread = dense ? -inner * inv_total : 0.f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = dense && total != 0.f ? -inner * (l[j] / total) : 0.f;
-    // Slot values: what slot r adds to its expert.
+    for (int j = 0; j < V; ++j) out[j] = dense ? spread * l[j] : 0.f;
+    // What each slot adds to its expert.
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
-      if (dense)
-        g[i] = p[i] * g[i];
-      else if (sigmoid) {
-        const float z = expf(-fabsf(c[i]));
-        g[i] = p[i] * ((c[i] > 0.f ? z : 1.f) / (1.f + z)) * (g[i] - (a.renormalize ? inner : 0.f));
-      } else {
-        g[i] = p[i] * (g[i] - inner);
+      if (L * i < a.k) {
+        if (dense)
+          g[i] = p[i] * g[i];
+        else if (sigmoid) {
+          const float z = expf(-fabsf(c[i]));
+          g[i] = p[i] * ((c[i] > 0.f ? z : 1.f) / (1.f + z)) * (g[i] - (a.renormalize ? inner : 0.f));
+        } else {
+          g[i] = p[i] * (g[i] - inner);
+        }
+        if (id[i] < 0) g[i] = 0.f;
       }
-      if (id[i] < 0) g[i] = 0.f;
     }
     for (int r = 0; r < a.k; ++r) {
       int e = -1;
@@ -378,15 +860,9 @@ __global__ void __launch_bounds__(kRouteThreads)
       v = __shfl_sync(0xffffffffu, v, src);
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (e == sub + L * j) out[j] += v;
+        if (e == sub * V + j) out[j] += v;
     }
-    if (live) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int e = sub + L * j;
-        if (e < a.n_experts) dl[t * a.n_experts + e] = Traits<T>::from_f(out[j]);
-      }
-    }
+    if (live) store_span<T, V>(dl + t * a.n_experts, sub * V, a.n_experts, vec, out);
   }
 }
 
@@ -406,9 +882,49 @@ unsigned route_grid(int64_t n, int lanes, int num_sms) {
   return static_cast<unsigned>(std::min<int64_t>((n + per_cta - 1) / per_cta, static_cast<int64_t>(num_sms) * 8));
 }
 
+template <typename T, int L, int V>
+cudaError_t launch_wide(const T* logits, const RouteArgs& a, int per, int32_t* idx, float* weights,
+                        cudaStream_t stream) {
+  const int smem = static_cast<int>(sizeof(WideSmem<L, V>)) * (kRouteThreads / 32) + L * WideSmem<L, V>::kLane * 4;
+  const int run = a.n_experts == L * V && reinterpret_cast<uintptr_t>(logits) % (4 * sizeof(T)) == 0;
+  const auto kernel = !a.bias && a.top_groups == a.n_groups ? route_wide_kernel<T, L, V, true> : route_wide_kernel<T, L, V, false>;
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+  if (e != cudaSuccess) return e;
+  const int64_t per_cta = kRouteThreads / L;
+  const int64_t ctas = (a.n + per_cta - 1) / per_cta;
+  if (ctas > INT32_MAX) return cudaErrorInvalidValue;
+  return launch_kernel(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kRouteThreads), smem, stream, logits, a, per, run,
+                       idx, weights);
+}
+
+// Lanes per token and experts per lane of the wide kernel, or false where it
+// does not apply: with groups, a lane holds a whole group or an equal part.
+bool wide_shape(const RouteArgs& a, int& lanes, int& per) {
+  if (a.k > kWideTopK || a.n_experts < 32) return false;
+  const bool grouped = a.top_groups < a.n_groups;
+  if (grouped && (a.n_groups & (a.n_groups - 1))) return false;
+  lanes = std::max(8, grouped ? a.n_groups : 8);
+  if (a.n_experts > 32 * lanes) lanes = 16;
+  if (grouped && a.n_experts % lanes) return false;
+  per = (a.n_experts + lanes - 1) / lanes;
+  return per <= 32;
+}
+
 template <typename T>
 cudaError_t route_t(const void* logits, const RouteArgs& a, int32_t* idx, float* weights, int num_sms,
                     cudaStream_t stream) {
+  int lanes, per;
+  if (wide_shape(a, lanes, per)) {
+    const T* x = static_cast<const T*>(logits);
+    if (lanes == 8)
+      return per <= 8    ? launch_wide<T, 8, 8>(x, a, per, idx, weights, stream)
+             : per <= 16 ? launch_wide<T, 8, 16>(x, a, per, idx, weights, stream)
+                         : launch_wide<T, 8, 32>(x, a, per, idx, weights, stream);
+    if (lanes == 16)
+      return per <= 16 ? launch_wide<T, 16, 16>(x, a, per, idx, weights, stream)
+                       : launch_wide<T, 16, 32>(x, a, per, idx, weights, stream);
+    return launch_wide<T, 32, 16>(x, a, per, idx, weights, stream);
+  }
   return by_width(a.n_experts, a.top_groups < a.n_groups, [&](auto l, auto v) {
     return launch_kernel(route_kernel<T, l.value, v.value>, dim3(route_grid(a.n, l.value, num_sms)),
                          dim3(kRouteThreads), 0, stream, static_cast<const T*>(logits), a, idx, weights);
@@ -418,11 +934,20 @@ cudaError_t route_t(const void* logits, const RouteArgs& a, int32_t* idx, float*
 template <typename T>
 cudaError_t route_backward_t(const float* dw, const void* logits, const int32_t* idx, const RouteArgs& a, void* dl,
                              int num_sms, cudaStream_t stream) {
-  return by_width(a.n_experts, false, [&](auto l, auto v) {
+  using std::integral_constant;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(dl);
+  const int vec = a.n_experts % 4 == 0 && at % (4 * sizeof(T)) == 0;
+  auto launch = [&](auto l, auto v) {
     return launch_kernel(route_backward_kernel<T, l.value, v.value>, dim3(route_grid(a.n, l.value, num_sms)),
-                         dim3(kRouteThreads), 0, stream, dw, static_cast<const T*>(logits), idx, a,
+                         dim3(kRouteThreads), 0, stream, dw, static_cast<const T*>(logits), idx, a, vec,
                          static_cast<T*>(dl));
-  });
+  };
+  const integral_constant<int, 8> v8;
+  if (a.n_experts <= 32) return launch(integral_constant<int, 4>{}, v8);
+  if (a.n_experts <= 64) return launch(integral_constant<int, 8>{}, v8);
+  if (a.n_experts <= 128) return launch(integral_constant<int, 16>{}, v8);
+  if (a.n_experts <= 256) return launch(integral_constant<int, 32>{}, v8);
+  return launch(integral_constant<int, 32>{}, integral_constant<int, 16>{});
 }
 
 }  // namespace

@@ -65,6 +65,40 @@ def test_groups_and_bias(n, E, k, groups, keep, dtype, score):
     check(x, k, score=score, bias=torch.zeros_like(b), n_groups=groups, top_groups=keep)
 
 
+@pytest.mark.parametrize("E", [32, 33, 48, 61, 64, 90, 96, 128, 130, 160, 200, 252, 256, 260, 384, 509, 512])
+def test_widths(E):
+    """Expert counts that do and do not divide among lanes, with aligned and unaligned rows, for k on both sides of 8."""
+    for dtype in (torch.float32, torch.bfloat16):
+        x = make(67, E, dtype, E)
+        b = torch.randn(E, generator=gen(E), device="cuda") * 0.1
+        for k in (1, 5, 8, 9):
+            check(x, k, score="sigmoid", bias=b)
+            check(x, k, score="softmax", renormalize=False)
+        for groups in (2, 4, 8, 16, 32):
+            if E % groups == 0:
+                for keep in {1, groups // 2}:
+                    k = min(8, E // groups)
+                    check(x, k, score="sigmoid", bias=b, n_groups=groups, top_groups=keep)
+                    check(x, k, score="softmax", n_groups=groups, top_groups=keep)
+        y = torch.empty(67 * E + 1, dtype=dtype, device="cuda")[1:].view(67, E).copy_(x)   # rows off their 16 bytes
+        check(y, 6, score="sigmoid", bias=b)
+        idx, w = ops.route_experts(y, 6)
+        assert torch.equal(ops.route_experts_backward(w, y, idx), ops.route_experts_backward(w, x, idx))
+
+
+def test_crowded_rows():
+    """Rows where many keys tie or nearly tie at the border, up to all of them."""
+    for E in (32, 64, 160, 256, 512):
+        x = torch.zeros(40, E, device="cuda")
+        x[:20] = torch.randint(0, 3, (20, E), generator=gen(E), device="cuda").float()
+        x[30:] = make(10, E, seed=E) * 1e-7
+        b = torch.randint(0, 2, (E,), generator=gen(1), device="cuda").float() * 0.25
+        for bias in (None, b, b + torch.arange(E, device="cuda") * 2.0 ** -24):
+            for score in ("softmax", "sigmoid"):
+                check(x, 8, score=score, bias=bias)
+                check(x, 8, score=score, bias=bias, n_groups=4, top_groups=2)
+
+
 def test_many_tokens():
     """Enough near ties that some need the second look in 64 bits."""
     for dtype in (torch.float32, torch.bfloat16):
