@@ -238,19 +238,24 @@ __device__ __forceinline__ void padded_prefix(const int* count_s, int E, int* st
   if (lane == 0) start_s[E] = carry;
 }
 
-// Small batches: every CTA counts all slots by itself and moves its share of
-// the tokens, one launch in all.
-constexpr int kSmallSlots = 2048;
+// Small batches: every CTA counts all slots by itself and its warps move
+// (token, 512 columns) units, one launch in all. The unit's elements are
+// loaded before the counting, which hides their latency.
+constexpr int kSmallSlots = 1024;
 template <typename T>
 __global__ void __launch_bounds__(kThreads) dispatch_small_kernel(Fp8Dispatch a, int width_k4) {
   __shared__ int idx_s[kSmallSlots];
   __shared__ int count_s[AGM_ROUTE_MAX_EXPERTS];
   __shared__ int start_s[AGM_ROUTE_MAX_EXPERTS + 1];
-  __shared__ int dest_s[kWarps][AGM_ROUTE_MAX_TOPK];
   const int lane = lane_id(), warp = warp_id();
   pdl_wait();
   pdl_trigger();
   const int slots = static_cast<int>(a.n) * a.k;
+  const int units = static_cast<int>(a.n) * width_k4;
+  int u = blockIdx.x * kWarps + warp;
+  float v[16];
+  if (u < units) load_unit<T>(static_cast<const T*>(a.x), u / width_k4, u % width_k4, a.d, lane, v);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.err = 0;
   for (int e = threadIdx.x; e < a.n_experts; e += kThreads) count_s[e] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < slots; i += kThreads) {
@@ -267,35 +272,35 @@ __global__ void __launch_bounds__(kThreads) dispatch_small_kernel(Fp8Dispatch a,
       a.counts[e] = count_s[e];
       a.seg_start[e] = start_s[e];
     }
-    if (threadIdx.x == 0) {
-      a.seg_start[a.n_experts] = start_s[a.n_experts];
-      if (start_s[a.n_experts] > a.max_rows) raise_error(a.err, kErrRowOverflow);
-    }
+    if (threadIdx.x == 0) a.seg_start[a.n_experts] = start_s[a.n_experts];
   }
-  for (int t = blockIdx.x * kWarps + warp; t < a.n; t += gridDim.x * kWarps) {
+  for (; u < units; u += gridDim.x * kWarps) {
+    const int t = u / width_k4, k4 = u - t * width_k4;
+    if (u >= static_cast<int>(gridDim.x) * kWarps) load_unit<T>(static_cast<const T*>(a.x), t, k4, a.d, lane, v);
+    uint32_t word;
+    const uint4 o = encode_unit(v, lane, word);
+    const int c = k4 * 512 + lane * 16;
     for (int r = 0; r < a.k; ++r) {
       const int s = t * a.k + r, e = idx_s[s];
       int before = 0;
       for (int i = lane; i < s; i += 32) before += idx_s[i] == e;
-      before = __reduce_add_sync(0xffffffffu, before);
-      if (lane == 0) {
-        const int64_t row = e >= 0 ? static_cast<int64_t>(start_s[e]) + before : -1;
-        dest_s[warp][r] = row < a.max_rows ? static_cast<int>(row) : -1;
-        a.row_of[s] = dest_s[warp][r];
-      }
+      const int64_t row = e >= 0 ? start_s[e] + static_cast<int>(__reduce_add_sync(0xffffffffu, before)) : -1;
+      if (k4 == 0 && lane == 0) a.row_of[s] = static_cast<int>(row);
+      if (row < 0) continue;
+      if (c < a.d) *reinterpret_cast<uint4*>(a.q + row * a.d + c) = o;
+      if (lane == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word_offset(row, k4, width_k4)) = word;
     }
-    __syncwarp();
-    scatter_row<T>(a, t, dest_s[warp], width_k4, lane);
-    __syncwarp();
   }
 }
 
 // Large batches, three launches. 1: per-expert counts of every 128 tokens.
 __global__ void __launch_bounds__(kThreads)
-    dispatch_hist_kernel(const int32_t* __restrict__ idx, int64_t slots, int k, int E, int32_t* __restrict__ hist) {
+    dispatch_hist_kernel(const int32_t* __restrict__ idx, int64_t slots, int k, int E, int32_t* __restrict__ hist,
+                         int* err) {
   __shared__ int count_s[AGM_ROUTE_MAX_EXPERTS];
   pdl_wait();
   pdl_trigger();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *err = 0;
   for (int e = threadIdx.x; e < E; e += kThreads) count_s[e] = 0;
   __syncthreads();
   const int64_t s0 = static_cast<int64_t>(blockIdx.x) * kTokBlk * k;
@@ -404,7 +409,9 @@ __global__ void __launch_bounds__(kThreads) dispatch_rows_kernel(Fp8Dispatch a, 
 // ---------------------------------------------------------------------------
 // Weighted sum
 // ---------------------------------------------------------------------------
-template <typename T>
+// One warp per (token, 256 columns): a lane sums 8 columns over the token's
+// rows, KU rows' loads in flight at a time.
+template <typename T, int KU>
 __global__ void __launch_bounds__(kThreads)
     combine_weighted_kernel(const T* __restrict__ y, const int32_t* __restrict__ row_of,
                             const float* __restrict__ weights, int64_t n, int nchunk, int k,
@@ -413,29 +420,41 @@ __global__ void __launch_bounds__(kThreads)
   pdl_trigger();
   const int lane = lane_id();
   const uint4* y4 = reinterpret_cast<const uint4*>(y);
+  const int parts = (nchunk + 31) / 32;
+  const int64_t units = n * parts;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + warp_id(); t < n; t += step) {
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + warp_id(); u < units; u += step) {
+    const int64_t t = u / parts;
+    const int c = static_cast<int>(u - t * parts) * 32 + lane;
     const int my_row = lane < k ? row_of[t * k + lane] : -1;
     const float my_w = lane < k ? weights[t * k + lane] : 0.f;
-    for (int c = lane; c - lane < nchunk; c += 32) {
-      float acc[8];
+    const bool in = c < nchunk;
+    float acc[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-      if (residual && c < nchunk) unpack8<T>(__ldcs(reinterpret_cast<const uint4*>(residual) + t * nchunk + c), acc);
-      for (int r = 0; r < k; ++r) {
-        const int row = __shfl_sync(0xffffffffu, my_row, r);
-        const float w = __shfl_sync(0xffffffffu, my_w, r);
-        if (row >= 0 && c < nchunk) {
-          float f[8];
-          unpack8<T>(__ldcs(y4 + static_cast<int64_t>(row) * nchunk + c), f);
+    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+    if (residual && in) unpack8<T>(__ldcs(reinterpret_cast<const uint4*>(residual) + t * nchunk + c), acc);
+    for (int r0 = 0; r0 < k; r0 += KU) {
+      uint4 v[KU];
+      float w[KU];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, f[i], acc[i]);
-        }
+      for (int i = 0; i < KU; ++i) {
+        const int row = __shfl_sync(0xffffffffu, my_row, (r0 + i) & 31);
+        w[i] = __shfl_sync(0xffffffffu, my_w, (r0 + i) & 31);
+        const bool use = r0 + i < k && row >= 0;
+        v[i] = use && in ? __ldcs(y4 + static_cast<int64_t>(row) * nchunk + c) : make_uint4(0, 0, 0, 0);
+        if (!use) w[i] = 0.f;  // a slot without a row adds nothing, whatever its weight
       }
-      if (c < nchunk)
-        reinterpret_cast<uint4*>(out)[t * nchunk + c] = make_uint4(pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3]),
-                                                                   pack2<T>(acc[4], acc[5]), pack2<T>(acc[6], acc[7]));
+#pragma unroll
+      for (int i = 0; i < KU; ++i) {
+        float f[8];
+        unpack8<T>(v[i], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = fmaf(w[i], f[j], acc[j]);
+      }
     }
+    if (in)
+      reinterpret_cast<uint4*>(out)[t * nchunk + c] = make_uint4(pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3]),
+                                                                 pack2<T>(acc[4], acc[5]), pack2<T>(acc[6], acc[7]));
   }
 }
 
@@ -448,10 +467,11 @@ template <typename T>
 cudaError_t dispatch_t(const Fp8Dispatch& a, int num_sms, cudaStream_t stream) {
   const int width_k4 = scale_k4(a.d);
   if (a.n * a.k <= kSmallSlots)
-    return launch_kernel(dispatch_small_kernel<T>, dim3(warp_grid(a.n, num_sms)), dim3(kThreads), 0, stream, a, width_k4);
+    return launch_kernel(dispatch_small_kernel<T>, dim3(warp_grid(a.n * width_k4, num_sms)), dim3(kThreads), 0,
+                         stream, a, width_k4);
   const int nb = static_cast<int>((a.n + kTokBlk - 1) / kTokBlk);
   cudaError_t e = launch_kernel(dispatch_hist_kernel, dim3(nb), dim3(kThreads), 0, stream, a.idx, a.n * a.k, a.k,
-                                a.n_experts, a.block_hist);
+                                a.n_experts, a.block_hist, a.err);
   if (e != cudaSuccess) return e;
   e = launch_kernel(dispatch_scan_kernel, dim3((a.n_experts + kWarps - 1) / kWarps), dim3(kThreads), 0, stream,
                     a.block_hist, nb, a.n_experts, a.counts);
@@ -527,14 +547,20 @@ cudaError_t dispatch_fp8(int dtype, const Fp8Dispatch& a, int num_sms, cudaStrea
 
 cudaError_t combine_weighted(int dtype, const void* y, const int32_t* row_of, const float* weights, int64_t n, int d,
                              int k, const void* residual, void* out, int num_sms, cudaStream_t stream) {
-  const dim3 grid(warp_grid(n, num_sms));
   const int nchunk = d / 8;
+  const dim3 grid(warp_grid(n * ((nchunk + 31) / 32), num_sms));
+  auto launch = [&](auto kernel, auto zero) {
+    using T = decltype(zero);
+    return launch_kernel(kernel, grid, dim3(kThreads), 0, stream, static_cast<const T*>(y), row_of, weights, n, nchunk, k,
+                         static_cast<const T*>(residual), static_cast<T*>(out));
+  };
   if (dtype == AGM_BF16)
-    return launch_kernel(combine_weighted_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, stream,
-                         static_cast<const __nv_bfloat16*>(y), row_of, weights, n, nchunk, k,
-                         static_cast<const __nv_bfloat16*>(residual), static_cast<__nv_bfloat16*>(out));
-  return launch_kernel(combine_weighted_kernel<__half>, grid, dim3(kThreads), 0, stream, static_cast<const __half*>(y),
-                       row_of, weights, n, nchunk, k, static_cast<const __half*>(residual), static_cast<__half*>(out));
+    return k <= 2   ? launch(combine_weighted_kernel<__nv_bfloat16, 2>, __nv_bfloat16())
+           : k <= 4 ? launch(combine_weighted_kernel<__nv_bfloat16, 4>, __nv_bfloat16())
+                    : launch(combine_weighted_kernel<__nv_bfloat16, 8>, __nv_bfloat16());
+  return k <= 2   ? launch(combine_weighted_kernel<__half, 2>, __half())
+         : k <= 4 ? launch(combine_weighted_kernel<__half, 4>, __half())
+                  : launch(combine_weighted_kernel<__half, 8>, __half());
 }
 
 }  // namespace agm

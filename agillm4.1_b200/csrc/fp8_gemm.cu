@@ -569,8 +569,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(tmem_slot, Cfg::kTmemCols);
     tmem_relinquish();
   }
-  pdl_wait();
-  pdl_trigger();
+  if (!args.early) {
+    pdl_wait();
+    pdl_trigger();
+  }
   load_groups(args, ROWS, grp);
   tc_fence_before();
   __syncthreads();
@@ -585,6 +587,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     int stage = 0;
     uint32_t phase = 0, armed = 0, armed_parity = 0;
     bool ok = true;
+    auto load_rows = [&](int st, int kb, const Unit& u, int boxes) {  // the elected lane
+      for (int i = 0; i < boxes; ++i)
+        tma_load_2d(sA + st * Cfg::kA + i * 32 * kBK, &tmA, kb * kBK, u.row0 + 32 * i, &full[st]);
+      if ((kb & 3) == 0) tma_load_3d(sSf + st * Cfg::kSf + kScaleTile, &tmSA, 0, kb >> 2, u.row0 >> 7, &full[st]);
+    };
+    // With `early`, the first unit's first stages get their weights before
+    // the wait for the previous kernel and their rows after it.
+    bool waited = !args.early;
+    int deferred = 0;
     for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
       const Unit u = weights_unit<ROWS>(grp, args.groups, t, num_n);
       const int boxes = (min(u.valid, ROWS) + 31) / 32;
@@ -598,13 +609,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool sf = (kb & 3) == 0;
           mbar_arrive_expect_tx(&full[stage], Cfg::kW + boxes * 32 * kBK + (sf ? Cfg::kSf : 0));
           tma_load_3d(sW + stage * Cfg::kW, &tmW, kb * kBK, u.nb * 128, u.g, &full[stage]);
-          for (int i = 0; i < boxes; ++i)
-            tma_load_2d(sA + stage * Cfg::kA + i * 32 * kBK, &tmA, kb * kBK, u.row0 + 32 * i, &full[stage]);
-          if (sf) {
-            uint8_t* dst = sSf + stage * Cfg::kSf;
-            tma_load_3d(dst, &tmSW, 0, kb >> 2, u.g * num_n + u.nb, &full[stage]);
-            tma_load_3d(dst + kScaleTile, &tmSA, 0, kb >> 2, u.row0 >> 7, &full[stage]);
-          }
+          if (sf) tma_load_3d(sSf + stage * Cfg::kSf, &tmSW, 0, kb >> 2, u.g * num_n + u.nb, &full[stage]);
+          if (waited) load_rows(stage, kb, u, boxes);
+        }
+        if (!waited && (++deferred == kStages || deferred == num_kb)) {
+          pdl_wait();
+          pdl_trigger();
+          waited = true;
+          if (elect_one())
+            for (int j = 0; j < deferred; ++j) load_rows(j, j, u, boxes);
         }
         armed |= 1u << stage;
         armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
@@ -614,6 +627,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           phase ^= 1;
         }
       }
+    }
+    if (!waited) {
+      // No unit (a unit's stages end the wait above): still order after the previous kernel.
+      pdl_wait();
+      pdl_trigger();
     }
     __syncwarp();
     for (int s = 0; s < kStages; ++s)

@@ -354,6 +354,10 @@ struct Fp8GemmArgs {
   int64_t live_rows = 0;           // host bound on the sum of the counts
   bool relu = false;
   bool zero_pad = false;           // write zeros to a segment's rows behind its count
+  // seg_start, counts, w and w_scales were written at least two launches ago,
+  // each of which waited for the one before it: they may be read, and the
+  // first weights loaded, before this launch waits for the previous one.
+  bool early = false;
   void* c = nullptr;               // [a_rows, n], c_dtype, or e4m3 when c_scales is set
   void* c_scales = nullptr;
   int* err = nullptr;

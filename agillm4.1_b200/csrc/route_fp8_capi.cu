@@ -240,8 +240,7 @@ int agm_moe_experts_fp8(const void* x, int dtype, int64_t n_tokens, int d, int n
   const void* ptrs[] = {x, w1, s1, b1, w2, s2, b2, residual, out, workspace};
   for (const void* p : ptrs)
     if (!aligned16(p)) return fail(AGM_ERR_ARG, "all tensors must be 16-byte aligned");
-  cudaError_t e = cudaMemsetAsync(L.err, 0, sizeof(int), stream);
-  if (e != cudaSuccess || n_tokens == 0) return done(e, "memset");
+  if (n_tokens == 0) return done(cudaMemsetAsync(L.err, 0, sizeof(int), stream), "memset");
   const int sms = num_sms();
   agm::Fp8Dispatch dsp;
   dsp.x = x;
@@ -258,7 +257,7 @@ int agm_moe_experts_fp8(const void* x, int dtype, int64_t n_tokens, int d, int n
   dsp.q = L.xq;
   dsp.scales = L.xs;
   dsp.err = L.err;
-  e = agm::dispatch_fp8(dtype, dsp, sms, stream);
+  cudaError_t e = agm::dispatch_fp8(dtype, dsp, sms, stream);  // clears the error word first
   if (e != cudaSuccess) return done(e, "dispatch_fp8");
   agm::Fp8GemmArgs g;
   g.a = L.xq;
@@ -289,6 +288,7 @@ int agm_moe_experts_fp8(const void* x, int dtype, int64_t n_tokens, int d, int n
   g.relu = false;
   g.c = L.y;
   g.c_scales = nullptr;
+  g.early = true;  // the segments come from the launches before FC1, the weights from before the call
   e = agm::grouped_gemm_fp8(dtype, g, AGM_FP8_AUTO, sms, stream);
   if (e != cudaSuccess) return done(e, "grouped_gemm_fp8 fc2");
   return done(agm::combine_weighted(dtype, L.y, L.row_of, weights, n_tokens, d, top_k, residual, out, sms, stream),

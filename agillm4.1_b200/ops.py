@@ -559,12 +559,14 @@ def moe_aux_backward(dloss: torch.Tensor, x: torch.Tensor, w_router: torch.Tenso
 def _call(dev: torch.device, name: str, *args) -> None:
     """Call a C entry point on ``dev``'s current stream, whichever device is current."""
     fn = getattr(load(), name)
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)  # a tenth of stream_handle()'s time
     if dev.index == torch.cuda.current_device():
-        rc = fn(*args, stream_handle(dev))
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, stream_handle(dev))
-    check(rc, name)
+            rc = fn(*args, stream)
+    if rc:
+        check(rc, name)
 
 
 def _need(what: str, t: torch.Tensor, dtype, shape, dev: torch.device) -> None:
