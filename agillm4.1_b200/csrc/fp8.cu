@@ -40,6 +40,39 @@ __device__ __forceinline__ void load16(const T* p, float (&v)[16]) {
   }
 }
 
+// The lane's 16 elements as they are in memory, so that several units can be in flight.
+template <typename T>
+struct Raw16 {
+  uint4 u[sizeof(T)];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) u[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void unpack(float (&v)[16]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[4 * i] = __uint_as_float(u[i].x);
+        v[4 * i + 1] = __uint_as_float(u[i].y);
+        v[4 * i + 2] = __uint_as_float(u[i].z);
+        v[4 * i + 3] = __uint_as_float(u[i].w);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float f[8];
+        unpack8<T>(u[i], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[8 * i + j] = f[j];
+      }
+    }
+  }
+};
+
 __device__ __forceinline__ float amax16(const float (&v)[16]) {
   float m = 0.f;
 #pragma unroll
@@ -198,25 +231,6 @@ __global__ void __launch_bounds__(kThreads)
 // ---------------------------------------------------------------------------
 // Dispatch
 // ---------------------------------------------------------------------------
-// Quantises token `tok`'s row once and writes it to the k rows dest[0 .. k).
-template <typename T>
-__device__ __forceinline__ void scatter_row(const Fp8Dispatch& a, int64_t tok, const int32_t* dest, int width_k4,
-                                            int lane) {
-  for (int k4 = 0; k4 < width_k4; ++k4) {
-    float v[16];
-    load_unit<T>(static_cast<const T*>(a.x), tok, k4, a.d, lane, v);
-    uint32_t word;
-    const uint4 o = encode_unit(v, lane, word);
-    const int c = k4 * 512 + lane * 16;
-    for (int r = 0; r < a.k; ++r) {
-      const int64_t row = dest[r];
-      if (row < 0) continue;
-      if (c < a.d) *reinterpret_cast<uint4*>(a.q + row * a.d + c) = o;
-      if (lane == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word_offset(row, k4, width_k4)) = word;
-    }
-  }
-}
-
 __device__ __forceinline__ int pad_rows(int count) { return (count + AGM_TILE_M - 1) / AGM_TILE_M * AGM_TILE_M; }
 
 // Exclusive prefix of the padded counts in count_s over E <= 512 experts, by
@@ -349,17 +363,19 @@ __global__ void __launch_bounds__(kThreads)
 
 // 3: destinations of a block's slots in slot order, then its rows. Each warp
 // ranks an eighth of the block's slots: matching lanes of 32 slots at a time,
-// on top of the counts of the warps before it.
+// on top of the counts of the warps before it. Small grids split a block's
+// rows over several CTAs, each of which ranks all its slots.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) dispatch_rows_kernel(Fp8Dispatch a, int width_k4) {
+__global__ void __launch_bounds__(kThreads) dispatch_rows_kernel(Fp8Dispatch a, int width_k4, int split) {
   __shared__ int start_s[AGM_ROUTE_MAX_EXPERTS + 1];
   __shared__ int base_s[kWarps][AGM_ROUTE_MAX_EXPERTS];
   __shared__ int32_t dest_s[kTokBlk * AGM_ROUTE_MAX_TOPK];
   const int lane = lane_id(), warp = warp_id();
   const int E = a.n_experts;
+  const int blk = blockIdx.x / split, part = blockIdx.x - blk * split;
   pdl_wait();
   pdl_trigger();
-  const int64_t tok0 = static_cast<int64_t>(blockIdx.x) * kTokBlk;
+  const int64_t tok0 = static_cast<int64_t>(blk) * kTokBlk;
   const int toks = static_cast<int>(min(static_cast<int64_t>(kTokBlk), a.n - tok0));
   const int slots = toks * a.k;
   const int per_warp = (slots + kWarps - 1) / kWarps;
@@ -374,7 +390,7 @@ __global__ void __launch_bounds__(kThreads) dispatch_rows_kernel(Fp8Dispatch a, 
   }
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += kThreads) {
-    int at = start_s[e] + a.block_hist[static_cast<int64_t>(blockIdx.x) * E + e];
+    int at = start_s[e] + a.block_hist[static_cast<int64_t>(blk) * E + e];
     for (int w = 0; w < kWarps; ++w) {
       const int c = base_s[w][e];
       base_s[w][e] = at;
@@ -397,21 +413,52 @@ __global__ void __launch_bounds__(kThreads) dispatch_rows_kernel(Fp8Dispatch a, 
     if (s < s1) {
       const int row = e >= 0 ? base + __popc(peers & ((1u << lane) - 1u)) : -1;
       dest_s[s] = row < a.max_rows ? row : -1;
-      a.row_of[tok0 * a.k + s] = dest_s[s];
+      if (part == 0) a.row_of[tok0 * a.k + s] = dest_s[s];
     }
     if (e >= 0 && lane == __ffs(peers) - 1) base_s[warp][e] = base + __popc(peers);
     __syncwarp();
   }
   __syncthreads();
-  for (int i = warp; i < toks; i += kWarps) scatter_row<T>(a, tok0 + i, dest_s + i * a.k, width_k4, lane);
+  // Rows: a warp takes a token, up to 4 x 512 columns in flight.
+  const T* x = static_cast<const T*>(a.x);
+  for (int i = part * kWarps + warp; i < toks; i += split * kWarps) {
+    const T* row = x + (tok0 + i) * a.d;
+    const int my_dest = lane < a.k ? dest_s[i * a.k + lane] : -1;
+    for (int q0 = 0; q0 < width_k4; q0 += 4) {
+      Raw16<T> raw[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = (q0 + q) * 512 + lane * 16;
+        if (c < a.d)
+          raw[q].load(row + c);
+        else
+          raw[q].clear();
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (q0 + q >= width_k4) break;
+        float v[16];
+        raw[q].unpack(v);
+        uint32_t word;
+        const uint4 o = encode_unit(v, lane, word);
+        const int c = (q0 + q) * 512 + lane * 16;
+        for (int r = 0; r < a.k; ++r) {
+          const int64_t to = __shfl_sync(0xffffffffu, my_dest, r);
+          if (to < 0) continue;
+          if (c < a.d) *reinterpret_cast<uint4*>(a.q + to * a.d + c) = o;
+          if (lane == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word_offset(to, q0 + q, width_k4)) = word;
+        }
+      }
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
 // Weighted sum
 // ---------------------------------------------------------------------------
-// One warp per (token, 256 columns): a lane sums 8 columns over the token's
-// rows, KU rows' loads in flight at a time.
-template <typename T, int KU>
+// One warp per token and P x 256 columns: a lane sums P x 8 columns over the
+// token's rows, the loads of KU rows in flight at a time.
+template <typename T, int KU, int P>
 __global__ void __launch_bounds__(kThreads)
     combine_weighted_kernel(const T* __restrict__ y, const int32_t* __restrict__ row_of,
                             const float* __restrict__ weights, int64_t n, int nchunk, int k,
@@ -420,41 +467,55 @@ __global__ void __launch_bounds__(kThreads)
   pdl_trigger();
   const int lane = lane_id();
   const uint4* y4 = reinterpret_cast<const uint4*>(y);
-  const int parts = (nchunk + 31) / 32;
+  const int parts = (nchunk + 32 * P - 1) / (32 * P);
   const int64_t units = n * parts;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
   for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + warp_id(); u < units; u += step) {
-    const int64_t t = u / parts;
-    const int c = static_cast<int>(u - t * parts) * 32 + lane;
+    const int64_t t = parts == 1 ? u : u / parts;
+    const int c0 = static_cast<int>(u - t * parts) * 32 * P + lane;
     const int my_row = lane < k ? row_of[t * k + lane] : -1;
     const float my_w = lane < k ? weights[t * k + lane] : 0.f;
-    const bool in = c < nchunk;
-    float acc[8];
+    float acc[P][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-    if (residual && in) unpack8<T>(__ldcs(reinterpret_cast<const uint4*>(residual) + t * nchunk + c), acc);
+    for (int p = 0; p < P; ++p) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[p][i] = 0.f;
+      const int c = c0 + 32 * p;
+      if (residual && c < nchunk) unpack8<T>(__ldcs(reinterpret_cast<const uint4*>(residual) + t * nchunk + c), acc[p]);
+    }
     for (int r0 = 0; r0 < k; r0 += KU) {
-      uint4 v[KU];
+      uint4 v[KU][P];
       float w[KU];
 #pragma unroll
       for (int i = 0; i < KU; ++i) {
         const int row = __shfl_sync(0xffffffffu, my_row, (r0 + i) & 31);
         w[i] = __shfl_sync(0xffffffffu, my_w, (r0 + i) & 31);
         const bool use = r0 + i < k && row >= 0;
-        v[i] = use && in ? __ldcs(y4 + static_cast<int64_t>(row) * nchunk + c) : make_uint4(0, 0, 0, 0);
         if (!use) w[i] = 0.f;  // a slot without a row adds nothing, whatever its weight
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          const int c = c0 + 32 * p;
+          v[i][p] = use && c < nchunk ? __ldcs(y4 + static_cast<int64_t>(row) * nchunk + c) : make_uint4(0, 0, 0, 0);
+        }
       }
 #pragma unroll
-      for (int i = 0; i < KU; ++i) {
-        float f[8];
-        unpack8<T>(v[i], f);
+      for (int i = 0; i < KU; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = fmaf(w[i], f[j], acc[j]);
-      }
+        for (int p = 0; p < P; ++p) {
+          float f[8];
+          unpack8<T>(v[i][p], f);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[p][j] = fmaf(w[i], f[j], acc[p][j]);
+        }
     }
-    if (in)
-      reinterpret_cast<uint4*>(out)[t * nchunk + c] = make_uint4(pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3]),
-                                                                 pack2<T>(acc[4], acc[5]), pack2<T>(acc[6], acc[7]));
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int c = c0 + 32 * p;
+      if (c < nchunk)
+        __stcs(reinterpret_cast<uint4*>(out) + t * nchunk + c,
+               make_uint4(pack2<T>(acc[p][0], acc[p][1]), pack2<T>(acc[p][2], acc[p][3]), pack2<T>(acc[p][4], acc[p][5]),
+                          pack2<T>(acc[p][6], acc[p][7])));
+    }
   }
 }
 
@@ -476,7 +537,9 @@ cudaError_t dispatch_t(const Fp8Dispatch& a, int num_sms, cudaStream_t stream) {
   e = launch_kernel(dispatch_scan_kernel, dim3((a.n_experts + kWarps - 1) / kWarps), dim3(kThreads), 0, stream,
                     a.block_hist, nb, a.n_experts, a.counts);
   if (e != cudaSuccess) return e;
-  return launch_kernel(dispatch_rows_kernel<T>, dim3(nb), dim3(kThreads), 0, stream, a, width_k4);
+  // At least four CTAs per SM, and at least one token per warp.
+  const int split = std::max(1, std::min(kTokBlk / kWarps, (4 * num_sms + nb - 1) / nb));
+  return launch_kernel(dispatch_rows_kernel<T>, dim3(nb * split), dim3(kThreads), 0, stream, a, width_k4, split);
 }
 
 }  // namespace
@@ -548,19 +611,23 @@ cudaError_t dispatch_fp8(int dtype, const Fp8Dispatch& a, int num_sms, cudaStrea
 cudaError_t combine_weighted(int dtype, const void* y, const int32_t* row_of, const float* weights, int64_t n, int d,
                              int k, const void* residual, void* out, int num_sms, cudaStream_t stream) {
   const int nchunk = d / 8;
-  const dim3 grid(warp_grid(n * ((nchunk + 31) / 32), num_sms));
-  auto launch = [&](auto kernel, auto zero) {
+  auto launch = [&](auto kernel, int columns, auto zero) {
     using T = decltype(zero);
-    return launch_kernel(kernel, grid, dim3(kThreads), 0, stream, static_cast<const T*>(y), row_of, weights, n, nchunk, k,
-                         static_cast<const T*>(residual), static_cast<T*>(out));
+    return launch_kernel(kernel, dim3(warp_grid(n * ((nchunk + columns - 1) / columns), num_sms)), dim3(kThreads), 0, stream,
+                         static_cast<const T*>(y), row_of, weights, n, nchunk, k, static_cast<const T*>(residual),
+                         static_cast<T*>(out));
   };
-  if (dtype == AGM_BF16)
-    return k <= 2   ? launch(combine_weighted_kernel<__nv_bfloat16, 2>, __nv_bfloat16())
-           : k <= 4 ? launch(combine_weighted_kernel<__nv_bfloat16, 4>, __nv_bfloat16())
-                    : launch(combine_weighted_kernel<__nv_bfloat16, 8>, __nv_bfloat16());
-  return k <= 2   ? launch(combine_weighted_kernel<__half, 2>, __half())
-         : k <= 4 ? launch(combine_weighted_kernel<__half, 4>, __half())
-                  : launch(combine_weighted_kernel<__half, 8>, __half());
+  // Few units: the narrowest, to use every SM. Many: enough loads in flight per warp.
+  auto pick = [&](auto zero) {
+    using T = decltype(zero);
+    const bool wide = n * ((nchunk + 31) / 32) >= static_cast<int64_t>(num_sms) * 64;
+    if (k <= 2)
+      return wide ? launch(combine_weighted_kernel<T, 2, 5>, 160, zero) : launch(combine_weighted_kernel<T, 2, 1>, 32, zero);
+    if (k <= 4)
+      return wide ? launch(combine_weighted_kernel<T, 4, 2>, 64, zero) : launch(combine_weighted_kernel<T, 4, 1>, 32, zero);
+    return launch(combine_weighted_kernel<T, 8, 1>, 32, zero);
+  };
+  return dtype == AGM_BF16 ? pick(__nv_bfloat16()) : pick(__half());
 }
 
 }  // namespace agm

@@ -167,7 +167,8 @@ template <typename OUT, bool RELU>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fp8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmSA,
-                    const __grid_constant__ CUtensorMap tmSB, Fp8GemmArgs args) {
+                    const __grid_constant__ CUtensorMap tmSB, const __grid_constant__ CUtensorMap tmA32,
+                    Fp8GemmArgs args) {
   constexpr bool OUT8 = sizeof(OUT) == 1;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Groups grp;
@@ -239,8 +240,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int t = cluster; t < total && ok; t += nclusters) {
       const Unit u = rows_unit(grp, args.groups, t, num_p, num_n);
-      // Rank 1 loads the block's second 128 rows (or repeats the first when there are none).
-      const int a_row = u.row0 + ((!leader && u.valid > 128) ? 128 : 0);
+      // Rank 1 loads the block's second 128 rows. Of a block that the group
+      // does not fill only the 32-row boxes with live rows are loaded: what
+      // stays in shared memory for the others reaches their own results only.
+      const int a_row = u.row0 + (leader ? 0 : 128);
+      const int boxes0 = min(4, (u.valid + 31) / 32), boxes1 = max(0, min(4, (u.valid - 97) / 32));
+      const int boxes = leader ? boxes0 : boxes1;
+      const uint32_t bytes = 2 * kPB + (boxes0 + boxes1) * 32 * kBK;
+      const uint32_t sf_bytes = 4 * kScaleTile + (boxes0 ? kScaleTile : 0) + (boxes1 ? kScaleTile : 0);
       const int n_mma = min(kPN, (args.n - u.nb * kPN + 31) / 32 * 32);
       const int b_row = u.nb * kPN + static_cast<int>(rank) * (n_mma / 2);
       for (int kb = 0; kb < num_kb; ++kb) {
@@ -251,13 +258,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         if (elect_one()) {
           const bool sf = (kb & 3) == 0;
-          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * (kPA + kPB + (sf ? kPSf : 0)));
+          if (leader) mbar_arrive_expect_tx(&full[stage], bytes + (sf ? sf_bytes : 0));
           const uint32_t fb = full0 + stage * 8;
           tma_load_3d_pair(sB + stage * kPB, &tmB, kb * kBK, b_row, u.g, fb);
-          tma_load_2d_pair(sA + stage * kPA, &tmA, kb * kBK, a_row, fb);
+          if (boxes == 4)
+            tma_load_2d_pair(sA + stage * kPA, &tmA, kb * kBK, a_row, fb);
+          else
+            for (int i = 0; i < boxes; ++i)
+              tma_load_2d_pair(sA + stage * kPA + i * 32 * kBK, &tmA32, kb * kBK, a_row + 32 * i, fb);
           if (sf) {
             uint8_t* dst = sSf + stage * kPSf;
-            tma_load_3d_pair(dst, &tmSA, 0, kb >> 2, a_row >> 7, fb);
+            if (boxes) tma_load_3d_pair(dst, &tmSA, 0, kb >> 2, a_row >> 7, fb);
             tma_load_3d_pair(dst + kScaleTile, &tmSB, 0, kb >> 2, u.g * w_tiles + 2 * u.nb, fb);
           }
         }
@@ -804,16 +815,19 @@ bool encode_scales(CUtensorMap* m, const void* base, int64_t tiles, int k4, int 
   return encode_tmap(m, base, 3, dims, str, box, CU_TENSOR_MAP_DATA_TYPE_UINT32, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-bool encode_operands(const Fp8GemmArgs& args, int a_box_rows, int w_tiles_box, CUtensorMap* tmA, CUtensorMap* tmW,
-                     CUtensorMap* tmSA, CUtensorMap* tmSW) {
+bool encode_rows(const Fp8GemmArgs& args, uint32_t box_rows, CUtensorMap* tmA) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(args.k), static_cast<uint64_t>(args.a_rows)};
+  const uint64_t str[1] = {static_cast<uint64_t>(args.k)};
+  const uint32_t box[2] = {kBK, box_rows};
+  return encode_tmap(tmA, args.a, 2, dims, str, box, CU_TENSOR_MAP_DATA_TYPE_UINT8);
+}
+
+// Both kernels' operands: rows in boxes of 32, weights in boxes of 128, scale tiles.
+bool encode_operands(const Fp8GemmArgs& args, int w_tiles_box, CUtensorMap* tmA, CUtensorMap* tmW, CUtensorMap* tmSA,
+                     CUtensorMap* tmSW) {
   const uint64_t k = static_cast<uint64_t>(args.k), n = static_cast<uint64_t>(args.n);
   const int k4 = scale_k4(args.k);
-  {
-    const uint64_t dims[2] = {k, static_cast<uint64_t>(args.a_rows)};
-    const uint64_t str[1] = {k};
-    const uint32_t box[2] = {kBK, static_cast<uint32_t>(a_box_rows)};
-    if (!encode_tmap(tmA, args.a, 2, dims, str, box, CU_TENSOR_MAP_DATA_TYPE_UINT8)) return false;
-  }
+  if (!encode_rows(args, 32, tmA)) return false;
   {
     const uint64_t dims[3] = {k, n, static_cast<uint64_t>(args.groups)};
     const uint64_t str[2] = {k, k * n};
@@ -826,8 +840,8 @@ bool encode_operands(const Fp8GemmArgs& args, int a_box_rows, int w_tiles_box, C
 
 template <typename OUT, bool RELU>
 cudaError_t launch_rows(const Fp8GemmArgs& args, int num_sms, cudaStream_t stream) {
-  CUtensorMap tmA, tmB, tmC, tmSA, tmSB;
-  if (!encode_operands(args, 128, 2, &tmA, &tmB, &tmSA, &tmSB)) return cudaErrorInvalidValue;
+  CUtensorMap tmA, tmA32, tmB, tmC, tmSA, tmSB;
+  if (!encode_operands(args, 2, &tmA32, &tmB, &tmSA, &tmSB) || !encode_rows(args, 128, &tmA)) return cudaErrorInvalidValue;
   {
     const uint64_t dims[2] = {static_cast<uint64_t>(args.n), static_cast<uint64_t>(args.a_rows)};
     const uint64_t str[1] = {static_cast<uint64_t>(args.n) * sizeof(OUT)};
@@ -840,13 +854,13 @@ cudaError_t launch_rows(const Fp8GemmArgs& args, int num_sms, cudaStream_t strea
   const int64_t units = (args.live_rows / 256 + args.groups) * static_cast<int64_t>((args.n + kPN - 1) / kPN);
   const int ctas = std::max(2, static_cast<int>(std::min<int64_t>(num_sms, 2 * units)) & ~1);
   return launch_kernel(fp8_rows_kernel<OUT, RELU>, dim3(ctas), dim3(kThreads), kPSmem, stream, tmA, tmB, tmC, tmSA,
-                       tmSB, args);
+                       tmSB, tmA32, args);
 }
 
 template <typename OUT, bool RELU, int ROWS>
 cudaError_t launch_weights(const Fp8GemmArgs& args, int num_sms, cudaStream_t stream) {
   CUtensorMap tmA, tmW, tmSA, tmSW;
-  if (!encode_operands(args, 32, 1, &tmA, &tmW, &tmSA, &tmSW)) return cudaErrorInvalidValue;
+  if (!encode_operands(args, 1, &tmA, &tmW, &tmSA, &tmSW)) return cudaErrorInvalidValue;
   const int smem = SwapCfg<ROWS>::kSmem;
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(fp8_weights_kernel<OUT, RELU, ROWS>), smem);
   if (e != cudaSuccess) return e;
