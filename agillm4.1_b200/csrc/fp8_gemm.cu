@@ -55,10 +55,12 @@ constexpr int kPA = 128 * kBK;                // 16 KB
 constexpr int kPB = 128 * kBK;                // 16 KB: half of the weight tile
 constexpr int kPSf = 3 * kScaleTile;          // scale tiles of a stage: a, and both halves of w
 constexpr int kPStg = 32 * 128;               // output chunk of one epilogue warp
+constexpr int kPBias = 128 * 4;               // its bias values
 constexpr int kAccStep = kPN - 32;            // second accumulator's first column
 constexpr int kSfCol = kAccStep + kPN;        // 480: two slots of 16 columns
 constexpr int kGroupPairs = 8;                // rasterisation: 8 row blocks per group of column tiles
-constexpr int kPSmem = kPStages * (kPA + kPB + kPSf) + kEpi * kPStg + 256 + 1024;
+constexpr int kPSmem = kPStages * (kPA + kPB + kPSf) + kEpi * (kPStg + kPBias) + 256 + 1024;
+static_assert(kPSmem + kMaxGroups * 12 + 16 <= 227 * 1024, "rows kernel shared memory");
 
 // ---- weights kernel ----
 template <int ROWS>
@@ -177,7 +179,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint8_t* sB = sA + kPStages * kPA;
   uint8_t* sStg = sB + kPStages * kPB;
   uint8_t* sSf = sStg + kEpi * kPStg;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sSf + kPStages * kPSf);  // rank 0's are used
+  float* sBias = reinterpret_cast<float*>(sSf + kPStages * kPSf);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sBias + kEpi * kPBias / 4);  // rank 0's are used
   uint64_t* empty = full + kPStages;                                    // both ranks
   uint64_t* acc_full = empty + kPStages;                                // both ranks
   uint64_t* acc_empty = acc_full + 2;                                   // rank 0's are used, as the rest
@@ -373,6 +376,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // the count are written (as zeros) when asked.
       const bool exists = leader || u.valid > 128;
       const bool work = exists && n_valid > 0 && (r_valid > 0 || args.zero_pad);
+      // The tile's bias values to shared memory while its products run: read
+      // from global memory at their use they cost a sixth of a short tile.
+      float* bias_s = sBias + ew * (kPBias / 4);
+      if (args.bias) {
+        const bool in = work && 4 * lane < n_valid;
+        const float4 b = in ? __ldg(reinterpret_cast<const float4*>(args.bias + static_cast<int64_t>(u.g) * args.n + n0) + lane)
+                            : make_float4(0.f, 0.f, 0.f, 0.f);
+        reinterpret_cast<float4*>(bias_s)[lane] = b;
+        __syncwarp();
+      }
       if (!mbar_wait(&acc_full[acc], (it >> 1) & 1, args.err, kErrTimeoutAcc) || *abort_s) {
         *abort_s = 1;
         break;
@@ -416,16 +429,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       if (!work) continue;
       const bool whole = r_valid >= 32 && n_valid >= 128;
-      const float* brow = args.bias ? args.bias + static_cast<int64_t>(u.g) * args.n + n0 : nullptr;
-      if (brow) {
+      if (args.bias) {
 #pragma unroll
         for (int q = 0; q < 32; ++q) {
-          if (whole || 4 * q < n_valid) {
-            const float4 b = __ldg(reinterpret_cast<const float4*>(brow + 4 * q));
-            add2(r[4 * q], r[4 * q + 1], b.x, b.y);
-            add2(r[4 * q + 2], r[4 * q + 3], b.z, b.w);
-          }
+          const float4 b = reinterpret_cast<const float4*>(bias_s)[q];
+          add2(r[4 * q], r[4 * q + 1], b.x, b.y);
+          add2(r[4 * q + 2], r[4 * q + 3], b.z, b.w);
         }
+        __syncwarp();  // before the next tile's values
       }
       if (RELU) {
 #pragma unroll
