@@ -18,28 +18,6 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTokBlk = AGM_DISPATCH_BLOCK;
 
-template <typename T>
-__device__ __forceinline__ void load16(const T* p, float (&v)[16]) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 f = __ldcs(reinterpret_cast<const float4*>(p) + i);
-      v[4 * i] = f.x;
-      v[4 * i + 1] = f.y;
-      v[4 * i + 2] = f.z;
-      v[4 * i + 3] = f.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float f[8];
-      unpack8<T>(__ldcs(reinterpret_cast<const uint4*>(p) + i), f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[8 * i + j] = f[j];
-    }
-  }
-}
-
 // The lane's 16 elements as they are in memory, so that several units can be in flight.
 template <typename T>
 struct Raw16 {
@@ -74,27 +52,50 @@ struct Raw16 {
 };
 
 __device__ __forceinline__ float amax16(const float (&v)[16]) {
+  float m[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m[i & 1] = fmaxf(m[i & 1], fabsf(v[i]));  // passes over NaN
+  return fmaxf(m[0], m[1]);
+}
+
+__device__ __forceinline__ bool is_inf(float v) { return v == __uint_as_float(0x7f800000u); }
+
+// The lane's values without infinities (as NaN), and their largest finite magnitude.
+__device__ __forceinline__ float drop_inf(float (&v)[16]) {
   float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) m = fmaxf(m, finite_abs(v[i]));
+  for (int i = 0; i < 16; ++i) {
+    m = fmaxf(m, finite_abs(v[i]));
+    v[i] = inf_to_nan(v[i]);
+  }
   return m;
 }
 
 __device__ __forceinline__ uint4 encode16(const float (&v)[16], float inv) {
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = pack_e4m3x4(inf_to_nan(v[4 * i]) * inv, inf_to_nan(v[4 * i + 1]) * inv, inf_to_nan(v[4 * i + 2]) * inv,
-                       inf_to_nan(v[4 * i + 3]) * inv);
+  for (int i = 0; i < 4; ++i) {
+    uint32_t x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = __float_as_uint(v[4 * i + j]);
+    scale2(x[0], x[1], inv);
+    scale2(x[2], x[3], inv);
+    w[i] = pack_e4m3x4(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3]));
+  }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Quantises the lane's 16 elements of 512 columns of a row; *word is the row's
+// Quantises the lane's 16 elements of 512 columns of a row; word is the row's
 // scale word (in every lane).
-__device__ __forceinline__ uint4 encode_unit(const float (&v)[16], int lane, uint32_t& word) {
+__device__ __forceinline__ uint4 encode_unit(float (&v)[16], int lane, uint32_t& word) {
   float m = amax16(v);
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (__any_sync(0xffffffffu, is_inf(m))) {
+    m = drop_inf(v);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  }
   const uint32_t byte = scale_byte(m);
   uint32_t w = byte << (8 * (lane >> 3));
   w |= __shfl_xor_sync(0xffffffffu, w, 8);
@@ -104,15 +105,35 @@ __device__ __forceinline__ uint4 encode_unit(const float (&v)[16], int lane, uin
 }
 
 template <typename T>
-__device__ __forceinline__ void load_unit(const T* x, int64_t row, int k4, int width, int lane, float (&v)[16]) {
+__device__ __forceinline__ void load_unit(const T* x, int64_t row, int k4, int width, int lane, Raw16<T>& raw) {
   const int c = k4 * 512 + lane * 16;
-  if (c < width) {
-    load16<T>(x + row * width + c, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = 0.f;
-  }
+  if (c < width)
+    raw.load(x + row * width + c);
+  else
+    raw.clear();
 }
+
+// Steps of a warp through the (row, 512 columns) units u, u + step, ...: one
+// division at the start, additions after it.
+struct UnitWalk {
+  int64_t row, step_rows;
+  int k4, step_k4, width_k4;
+  __device__ __forceinline__ UnitWalk(int64_t u, int64_t step, int width_k4_)
+      : row(u / width_k4_), step_rows(step / width_k4_), width_k4(width_k4_) {
+    k4 = static_cast<int>(u - row * width_k4);
+    step_k4 = static_cast<int>(step - step_rows * width_k4);
+  }
+  __device__ __forceinline__ void next() {
+    row += step_rows;
+    k4 += step_k4;
+    if (k4 >= width_k4) {
+      k4 -= width_k4;
+      ++row;
+    }
+  }
+};
+
+constexpr int kFlight = 4;  // units of a warp in flight
 
 // One warp per (row, 512 columns); rows up to the next multiple of 128 get a
 // scale word only, so that whole scale tiles are defined.
@@ -121,20 +142,33 @@ __global__ void __launch_bounds__(kThreads)
     quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int width, int width_k4, uint8_t* __restrict__ q,
                          uint8_t* __restrict__ scales) {
   const int lane = lane_id();
-  const int64_t units = (rows + 127) / 128 * 128 * width_k4;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + warp_id(); u < units; u += step) {
-    const int64_t row = u / width_k4;
-    const int k4 = static_cast<int>(u - row * width_k4);
-    uint32_t word = 0;
-    if (row < rows) {
-      float v[16];
-      load_unit<T>(x, row, k4, width, lane, v);
-      const uint4 o = encode_unit(v, lane, word);
-      const int c = k4 * 512 + lane * 16;
-      if (c < width) *reinterpret_cast<uint4*>(q + row * width + c) = o;
+  const int64_t all_rows = (rows + 127) / 128 * 128;
+  UnitWalk w(static_cast<int64_t>(blockIdx.x) * kWarps + warp_id(), static_cast<int64_t>(gridDim.x) * kWarps, width_k4);
+  while (w.row < all_rows) {
+    Raw16<T> raw[kFlight];
+    UnitWalk ahead = w;
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      const int c = ahead.k4 * 512 + lane * 16;
+      if (ahead.row < rows && c < width)
+        raw[i].load(x + ahead.row * width + c);
+      else
+        raw[i].clear();
+      ahead.next();
     }
-    if (lane == 0) *reinterpret_cast<uint32_t*>(scales + scale_word_offset(row, k4, width_k4)) = word;
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      if (w.row < all_rows) {
+        float v[16];
+        raw[i].unpack(v);
+        uint32_t word;
+        const uint4 o = encode_unit(v, lane, word);
+        const int c = w.k4 * 512 + lane * 16;
+        if (w.row < rows && c < width) *reinterpret_cast<uint4*>(q + w.row * width + c) = o;
+        if (lane == 0) *reinterpret_cast<uint32_t*>(scales + scale_word_offset(w.row, w.k4, width_k4)) = word;
+      }
+      w.next();
+    }
   }
 }
 
@@ -151,30 +185,49 @@ __global__ void __launch_bounds__(kThreads)
   const int lane = lane_id(), sub = threadIdx.x & 7, r0 = threadIdx.x >> 3;
   const int c = kb * 128 + sub * 16;
   const int64_t base = g * n;
-  float v[4][16], m = 0.f;
+  Raw16<T> raw[4];
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     const int r = nb * 128 + p * 32 + r0;
-    if (r < n && c < width) {
-      load16<T>(w + (base + r) * width + c, v[p]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[p][i] = 0.f;
-    }
-    m = fmaxf(m, amax16(v[p]));
+    if (r < n && c < width)
+      raw[p].load(w + (base + r) * width + c);
+    else
+      raw[p].clear();
   }
+  float m = 0.f, v[16];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) max_s[warp_id()] = m;
-  __syncthreads();
+  for (int p = 0; p < 4; ++p) {
+    raw[p].unpack(v);
+    m = fmaxf(m, amax16(v));
+  }
+  auto block_max = [&]() {
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) m = fmaxf(m, max_s[i]);
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) max_s[warp_id()] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) m = fmaxf(m, max_s[i]);
+  };
+  block_max();
+  const bool odd = is_inf(m);  // the same in every thread
+  if (odd) {
+    __syncthreads();
+    m = 0.f;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      raw[p].unpack(v);
+      m = fmaxf(m, drop_inf(v));
+    }
+    block_max();
+  }
   const uint32_t byte = scale_byte(m);
   const float inv = inv_scale(byte);
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     const int r = nb * 128 + p * 32 + r0;
-    if (r < n && c < width) *reinterpret_cast<uint4*>(q + (base + r) * width + c) = encode16(v[p], inv);
+    raw[p].unpack(v);
+    if (odd) drop_inf(v);
+    if (r < n && c < width) *reinterpret_cast<uint4*>(q + (base + r) * width + c) = encode16(v, inv);
   }
   // Every row of the tile gets the block's byte; the last block also clears
   // the bytes of the K blocks that do not exist.
@@ -189,41 +242,58 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 template <typename T>
+__device__ __forceinline__ void decode_unit(const uint4& b, uint32_t word, int lane, T* __restrict__ o) {
+  const float s = scale_value((word >> (8 * (lane >> 3))) & 0xffu);
+  const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = unpack_e4m3x2(bw[i >> 1] >> (16 * (i & 1)));
+    v[2 * i] = f.x * s;
+    v[2 * i + 1] = f.y * s;
+  }
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      __stcs(reinterpret_cast<float4*>(o) + i, make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      __stcs(reinterpret_cast<uint4*>(o) + i,
+             make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
+                        pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7])));
+  }
+}
+
+// Rows of all groups in one sequence; a group's scale tiles start anew.
+template <typename T>
 __global__ void __launch_bounds__(kThreads)
     dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales, int64_t groups, int64_t rows,
                       int width, int width_k4, T* __restrict__ out) {
   const int lane = lane_id();
   const int64_t tile_rows = (rows + 127) / 128 * 128;
-  const int64_t units = groups * rows * width_k4;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + warp_id(); u < units; u += step) {
-    const int64_t gr = u / width_k4;
-    const int k4 = static_cast<int>(u - gr * width_k4);
-    const int64_t g = gr / rows;
-    const int64_t r = gr - g * rows;
-    const int c = k4 * 512 + lane * 16;
-    if (c >= width) continue;
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(scales + scale_word_offset(g * tile_rows + r, k4, width_k4));
-    const float s = scale_value((word >> (8 * (lane >> 3))) & 0xffu);
-    const uint4 b = __ldcs(reinterpret_cast<const uint4*>(q + gr * width + c));
-    const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
-    float v[16];
+  const int64_t all_rows = groups * rows;
+  UnitWalk w(static_cast<int64_t>(blockIdx.x) * kWarps + warp_id(), static_cast<int64_t>(gridDim.x) * kWarps, width_k4);
+  while (w.row < all_rows) {
+    uint4 b[kFlight];
+    uint32_t word[kFlight];
+    UnitWalk ahead = w;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 f = unpack_e4m3x2(bw[i >> 1] >> (16 * (i & 1)));
-      v[2 * i] = f.x * s;
-      v[2 * i + 1] = f.y * s;
+    for (int i = 0; i < kFlight; ++i) {
+      const int c = ahead.k4 * 512 + lane * 16;
+      if (ahead.row < all_rows && c < width) {
+        const int64_t g = groups == 1 ? 0 : ahead.row / rows;
+        word[i] = __ldg(reinterpret_cast<const uint32_t*>(
+            scales + scale_word_offset(g * tile_rows + ahead.row - g * rows, ahead.k4, width_k4)));
+        b[i] = __ldcs(reinterpret_cast<const uint4*>(q + ahead.row * width + c));
+      }
+      ahead.next();
     }
-    T* o = out + gr * width + c;
-    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        reinterpret_cast<float4*>(o)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        reinterpret_cast<uint4*>(o)[i] = make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
-                                                    pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
+    for (int i = 0; i < kFlight; ++i) {
+      const int c = w.k4 * 512 + lane * 16;
+      if (w.row < all_rows && c < width) decode_unit<T>(b[i], word[i], lane, out + w.row * width + c);
+      w.next();
     }
   }
 }
@@ -267,8 +337,8 @@ __global__ void __launch_bounds__(kThreads) dispatch_small_kernel(Fp8Dispatch a,
   const int slots = static_cast<int>(a.n) * a.k;
   const int units = static_cast<int>(a.n) * width_k4;
   int u = blockIdx.x * kWarps + warp;
-  float v[16];
-  if (u < units) load_unit<T>(static_cast<const T*>(a.x), u / width_k4, u % width_k4, a.d, lane, v);
+  Raw16<T> raw;
+  if (u < units) load_unit<T>(static_cast<const T*>(a.x), u / width_k4, u % width_k4, a.d, lane, raw);
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.err = 0;
   for (int e = threadIdx.x; e < a.n_experts; e += kThreads) count_s[e] = 0;
   __syncthreads();
@@ -290,7 +360,9 @@ __global__ void __launch_bounds__(kThreads) dispatch_small_kernel(Fp8Dispatch a,
   }
   for (; u < units; u += gridDim.x * kWarps) {
     const int t = u / width_k4, k4 = u - t * width_k4;
-    if (u >= static_cast<int>(gridDim.x) * kWarps) load_unit<T>(static_cast<const T*>(a.x), t, k4, a.d, lane, v);
+    if (u >= static_cast<int>(gridDim.x) * kWarps) load_unit<T>(static_cast<const T*>(a.x), t, k4, a.d, lane, raw);
+    float v[16];
+    raw.unpack(v);
     uint32_t word;
     const uint4 o = encode_unit(v, lane, word);
     const int c = k4 * 512 + lane * 16;

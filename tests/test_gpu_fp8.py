@@ -90,6 +90,17 @@ def test_quantize_non_finite_stays_visible_and_alone(bad):
     torch.testing.assert_close(got.double(), fo.values(q, p), rtol=0, atol=0, equal_nan=True)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantize_weight_non_finite(dtype):
+    w = weight(2, 200, 272, 3, dtype)
+    w[0, 5, 7], w[0, 130, 200], w[1, 199, 271] = float("inf"), float("nan"), -float("inf")
+    t = ops.quantize_fp8_weight(w)
+    q, p = fo.quantize(w.double(), 128)
+    got = ops.dequantize_fp8(t, torch.float32)
+    assert int(torch.isnan(got).sum()) == 3
+    torch.testing.assert_close(got.double(), fo.values(q, fo.row_exponents(p, 200, 128)), rtol=0, atol=0, equal_nan=True)
+
+
 # ---------------------------------------------------------------------------
 # Grouped product
 # ---------------------------------------------------------------------------
