@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kThreads)
 // on top of the counts of the warps before it. Small grids split a block's
 // rows over several CTAs, each of which ranks all its slots.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) dispatch_rows_kernel(Fp8Dispatch a, int width_k4, int split) {
+__global__ void __launch_bounds__(kThreads, 3) dispatch_rows_kernel(Fp8Dispatch a, int width_k4, int split) {
   __shared__ int start_s[AGM_ROUTE_MAX_EXPERTS + 1];
   __shared__ int base_s[kWarps][AGM_ROUTE_MAX_EXPERTS];
   __shared__ int32_t dest_s[kTokBlk * AGM_ROUTE_MAX_TOPK];
@@ -453,6 +453,14 @@ __global__ void __launch_bounds__(kThreads) dispatch_rows_kernel(Fp8Dispatch a, 
   const int per_warp = (slots + kWarps - 1) / kWarps;
   const int s0 = min(slots, warp * per_warp), s1 = min(slots, s0 + per_warp);
   const int32_t* idx = a.idx + tok0 * a.k;
+  auto load_four = [&](int tok, int k4, Raw16<T>(&to)[4]) {
+    const T* row = static_cast<const T*>(a.x) + (tok0 + tok) * a.d;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) load_unit<T>(row, 0, k4 + q, a.d, lane, to[q]);
+  };
+  const int first = part * kWarps + warp;
+  Raw16<T> raw[4];
+  if (first < toks) load_four(first, 0, raw);  // in flight during the ranking
   if (warp == 0) padded_prefix(a.counts, E, start_s, lane);
   for (int e = lane; e < E; e += 32) base_s[warp][e] = 0;
   __syncwarp();
@@ -491,37 +499,38 @@ __global__ void __launch_bounds__(kThreads) dispatch_rows_kernel(Fp8Dispatch a, 
     __syncwarp();
   }
   __syncthreads();
-  // Rows: a warp takes a token, up to 4 x 512 columns in flight.
-  const T* x = static_cast<const T*>(a.x);
-  for (int i = part * kWarps + warp; i < toks; i += split * kWarps) {
-    const T* row = x + (tok0 + i) * a.d;
+  // Rows: a warp takes a token, 4 x 512 columns at a time, the next ones in
+  // flight while these are rounded and written.
+  int i = first;
+  int q0 = 0;
+  while (i < toks) {
+    int ni = i, nq = q0 + 4;
+    if (nq >= width_k4) {
+      nq = 0;
+      ni += split * kWarps;
+    }
+    Raw16<T> next[4];
+    if (ni < toks) load_four(ni, nq, next);
     const int my_dest = lane < a.k ? dest_s[i * a.k + lane] : -1;
-    for (int q0 = 0; q0 < width_k4; q0 += 4) {
-      Raw16<T> raw[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = (q0 + q) * 512 + lane * 16;
-        if (c < a.d)
-          raw[q].load(row + c);
-        else
-          raw[q].clear();
-      }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (q0 + q >= width_k4) break;
-        float v[16];
-        raw[q].unpack(v);
-        uint32_t word;
-        const uint4 o = encode_unit(v, lane, word);
-        const int c = (q0 + q) * 512 + lane * 16;
-        for (int r = 0; r < a.k; ++r) {
-          const int64_t to = __shfl_sync(0xffffffffu, my_dest, r);
-          if (to < 0) continue;
-          if (c < a.d) *reinterpret_cast<uint4*>(a.q + to * a.d + c) = o;
-          if (lane == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word_offset(to, q0 + q, width_k4)) = word;
-        }
+    for (int q = 0; q < 4; ++q) {
+      if (q0 + q >= width_k4) break;
+      float v[16];
+      raw[q].unpack(v);
+      uint32_t word;
+      const uint4 o = encode_unit(v, lane, word);
+      const int c = (q0 + q) * 512 + lane * 16;
+      for (int r = 0; r < a.k; ++r) {
+        const int64_t to = __shfl_sync(0xffffffffu, my_dest, r);
+        if (to < 0) continue;
+        if (c < a.d) *reinterpret_cast<uint4*>(a.q + to * a.d + c) = o;
+        if (lane == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word_offset(to, q0 + q, width_k4)) = word;
       }
     }
+    i = ni;
+    q0 = nq;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) raw[q] = next[q];
   }
 }
 
@@ -529,16 +538,19 @@ __global__ void __launch_bounds__(kThreads) dispatch_rows_kernel(Fp8Dispatch a, 
 // Weighted sum
 // ---------------------------------------------------------------------------
 // One warp per token and P x 256 columns: a lane sums P x 8 columns over the
-// token's rows, the loads of KU rows in flight at a time.
-template <typename T, int KU, int P>
+// token's rows, the loads of KU rows in flight at a time. ONE: k <= KU, so
+// that only one part's sums are held at a time.
+template <typename T, int KU, int P, bool ONE>
 __global__ void __launch_bounds__(kThreads)
     combine_weighted_kernel(const T* __restrict__ y, const int32_t* __restrict__ row_of,
                             const float* __restrict__ weights, int64_t n, int nchunk, int k,
                             const T* __restrict__ residual, T* __restrict__ out) {
+  static_assert(ONE || P == 1, "several parts only for few rows");
   pdl_wait();
   pdl_trigger();
   const int lane = lane_id();
   const uint4* y4 = reinterpret_cast<const uint4*>(y);
+  const uint4* res4 = reinterpret_cast<const uint4*>(residual);
   const int parts = (nchunk + 32 * P - 1) / (32 * P);
   const int64_t units = n * parts;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
@@ -547,15 +559,26 @@ __global__ void __launch_bounds__(kThreads)
     const int c0 = static_cast<int>(u - t * parts) * 32 * P + lane;
     const int my_row = lane < k ? row_of[t * k + lane] : -1;
     const float my_w = lane < k ? weights[t * k + lane] : 0.f;
-    float acc[P][8];
+    float acc[8];
+    auto start = [&](int c) {
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
+      for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+      if (residual && c < nchunk) unpack8<T>(__ldcs(res4 + t * nchunk + c), acc);
+    };
+    auto add = [&](const uint4& v, float w) {
+      float f[8];
+      unpack8<T>(v, f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[p][i] = 0.f;
-      const int c = c0 + 32 * p;
-      if (residual && c < nchunk) unpack8<T>(__ldcs(reinterpret_cast<const uint4*>(residual) + t * nchunk + c), acc[p]);
-    }
-    for (int r0 = 0; r0 < k; r0 += KU) {
+      for (int j = 0; j < 8; ++j) acc[j] = fmaf(w, f[j], acc[j]);
+    };
+    auto finish = [&](int c) {
+      if (c < nchunk)
+        __stcs(reinterpret_cast<uint4*>(out) + t * nchunk + c,
+               make_uint4(pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3]), pack2<T>(acc[4], acc[5]),
+                          pack2<T>(acc[6], acc[7])));
+    };
+    if (!ONE) start(c0);
+    for (int r0 = 0; r0 < (ONE ? 1 : k); r0 += KU) {
       uint4 v[KU][P];
       float w[KU];
 #pragma unroll
@@ -570,24 +593,20 @@ __global__ void __launch_bounds__(kThreads)
           v[i][p] = use && c < nchunk ? __ldcs(y4 + static_cast<int64_t>(row) * nchunk + c) : make_uint4(0, 0, 0, 0);
         }
       }
-#pragma unroll
-      for (int i = 0; i < KU; ++i)
+      if constexpr (ONE) {
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-          float f[8];
-          unpack8<T>(v[i][p], f);
+          start(c0 + 32 * p);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) acc[p][j] = fmaf(w[i], f[j], acc[p][j]);
+          for (int i = 0; i < KU; ++i) add(v[i][p], w[i]);
+          finish(c0 + 32 * p);
         }
-    }
+      } else {
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const int c = c0 + 32 * p;
-      if (c < nchunk)
-        __stcs(reinterpret_cast<uint4*>(out) + t * nchunk + c,
-               make_uint4(pack2<T>(acc[p][0], acc[p][1]), pack2<T>(acc[p][2], acc[p][3]), pack2<T>(acc[p][4], acc[p][5]),
-                          pack2<T>(acc[p][6], acc[p][7])));
+        for (int i = 0; i < KU; ++i) add(v[i][0], w[i]);
+      }
     }
+    if (!ONE) finish(c0);
   }
 }
 
@@ -694,10 +713,12 @@ cudaError_t combine_weighted(int dtype, const void* y, const int32_t* row_of, co
     using T = decltype(zero);
     const bool wide = n * ((nchunk + 31) / 32) >= static_cast<int64_t>(num_sms) * 64;
     if (k <= 2)
-      return wide ? launch(combine_weighted_kernel<T, 2, 5>, 160, zero) : launch(combine_weighted_kernel<T, 2, 1>, 32, zero);
+      return wide ? launch(combine_weighted_kernel<T, 2, 5, true>, 160, zero)
+                  : launch(combine_weighted_kernel<T, 2, 1, true>, 32, zero);
     if (k <= 4)
-      return wide ? launch(combine_weighted_kernel<T, 4, 2>, 64, zero) : launch(combine_weighted_kernel<T, 4, 1>, 32, zero);
-    return launch(combine_weighted_kernel<T, 8, 1>, 32, zero);
+      return wide ? launch(combine_weighted_kernel<T, 4, 2, true>, 64, zero)
+                  : launch(combine_weighted_kernel<T, 4, 1, true>, 32, zero);
+    return launch(combine_weighted_kernel<T, 8, 1, false>, 32, zero);
   };
   return dtype == AGM_BF16 ? pick(__nv_bfloat16()) : pick(__half());
 }
