@@ -339,7 +339,10 @@ __global__ void __launch_bounds__(kThreads) dispatch_small_kernel(Fp8Dispatch a,
   int u = blockIdx.x * kWarps + warp;
   Raw16<T> raw;
   if (u < units) load_unit<T>(static_cast<const T*>(a.x), u / width_k4, u % width_k4, a.d, lane, raw);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.err = 0;
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) *a.err = 0;
+    for (int i = threadIdx.x; i < a.n_zero; i += kThreads) a.zero[i] = 0;
+  }
   for (int e = threadIdx.x; e < a.n_experts; e += kThreads) count_s[e] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < slots; i += kThreads) {
@@ -382,11 +385,14 @@ __global__ void __launch_bounds__(kThreads) dispatch_small_kernel(Fp8Dispatch a,
 // Large batches, three launches. 1: per-expert counts of every 128 tokens.
 __global__ void __launch_bounds__(kThreads)
     dispatch_hist_kernel(const int32_t* __restrict__ idx, int64_t slots, int k, int E, int32_t* __restrict__ hist,
-                         int* err) {
+                         int* err, int32_t* __restrict__ zero, int n_zero) {
   __shared__ int count_s[AGM_ROUTE_MAX_EXPERTS];
   pdl_wait();
   pdl_trigger();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *err = 0;
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) *err = 0;
+    for (int i = threadIdx.x; i < n_zero; i += kThreads) zero[i] = 0;
+  }
   for (int e = threadIdx.x; e < E; e += kThreads) count_s[e] = 0;
   __syncthreads();
   const int64_t s0 = static_cast<int64_t>(blockIdx.x) * kTokBlk * k;
@@ -623,7 +629,7 @@ cudaError_t dispatch_t(const Fp8Dispatch& a, int num_sms, cudaStream_t stream) {
                          stream, a, width_k4);
   const int nb = static_cast<int>((a.n + kTokBlk - 1) / kTokBlk);
   cudaError_t e = launch_kernel(dispatch_hist_kernel, dim3(nb), dim3(kThreads), 0, stream, a.idx, a.n * a.k, a.k,
-                                a.n_experts, a.block_hist, a.err);
+                                a.n_experts, a.block_hist, a.err, a.zero, a.n_zero);
   if (e != cudaSuccess) return e;
   e = launch_kernel(dispatch_scan_kernel, dim3((a.n_experts + kWarps - 1) / kWarps), dim3(kThreads), 0, stream,
                     a.block_hist, nb, a.n_experts, a.counts);

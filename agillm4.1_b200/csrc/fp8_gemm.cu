@@ -24,9 +24,20 @@
 //   epilogue's arithmetic.
 //
 // * fp8_weights_kernel, few rows per group (bound by reading the weights): the
-//   weight tile is the 128-row operand and the group's rows the N operand (32
-//   of them, or up to 128), so no bandwidth goes to padding rows and the ring
-//   of stages keeps 144 KB of weights in flight per SM.
+//   weight tile is the 128-row operand and up to 128 of the group's rows the N
+//   operand, of which only the 32-row boxes with live rows are loaded and
+//   multiplied. The ring keeps 96 KB of weights in flight per SM; 144 KB, with
+//   room for 32 rows only, was not faster at 8 rows per group (42 against 40
+//   us for 61 x 1488 x 2000) and slower from 32 on.
+//
+//   It also runs both products of a block of experts in one launch: units of
+//   the first product, then of the second, are drawn from a ticket counter.
+//   A unit of the second waits until all columns of its rows have been
+//   written (a counter per 128-row block), after its first weights are on
+//   their way, so the weights stream through the change from one product to
+//   the other. Tickets keep this free of deadlocks whatever part of the grid
+//   is running: a unit that is waited for was drawn earlier, by a CTA that
+//   runs and waits for nothing but units drawn before.
 //
 // Both walk units numbered from the device-side row counts (no host sync;
 // empty groups cost nothing), are persistent and warp-specialised (warp 0 TMA,
@@ -63,18 +74,16 @@ constexpr int kPSmem = kPStages * (kPA + kPB + kPSf) + kEpi * (kPStg + kPBias) +
 static_assert(kPSmem + kMaxGroups * 12 + 16 <= 227 * 1024, "rows kernel shared memory");
 
 // ---- weights kernel ----
-template <int ROWS>
-struct SwapCfg {
-  static constexpr int kStages = ROWS == 32 ? 9 : 6;
-  static constexpr int kW = 128 * kBK;
-  static constexpr int kA = ROWS * kBK;
-  static constexpr int kSf = 2 * kScaleTile;
-  static constexpr int kStgLd = 132;          // floats per staged row
-  static constexpr int kStg = 32 * kStgLd * 4;
-  static constexpr int kTmemCols = ROWS == 32 ? 128 : 512;
-  static constexpr int kSfCol = 2 * ROWS;
-  static constexpr int kSmem = kStages * (kW + kA + kSf) + kStg + 512 + 1024;
-};
+constexpr int kWStages = 6;
+constexpr int kWRows = 128;                   // rows of a unit
+constexpr int kWW = 128 * kBK;                // 16 KB of weights
+constexpr int kWA = kWRows * kBK;
+constexpr int kWSf = 2 * kScaleTile;
+constexpr int kWStgLd = 132;                  // floats per staged row
+constexpr int kWStg = 32 * kWStgLd * 4;
+constexpr int kWSfCol = 2 * kWRows;           // behind the two accumulators: two slots of 8 columns
+constexpr int kWQueue = 4;                    // units drawn ahead
+constexpr int kWSmem = kWStages * (kWW + kWA + kWSf) + kWStg + 512 + 1024;
 
 // Row counts and starts of the groups, checked, and the prefix sum of their
 // blocks of `ROWS` rows.
@@ -152,15 +161,13 @@ __device__ __forceinline__ Unit rows_unit(const Groups& s, int groups, int t, in
   return u;
 }
 
-template <int ROWS>
-__device__ __forceinline__ Unit weights_unit(const Groups& s, int groups, int t, int num_n) {
-  const int b = t / num_n;
+__device__ __forceinline__ Unit weights_unit(const Groups& s, int groups, int b, int nb) {
   Unit u;
-  u.nb = t - b * num_n;
+  u.nb = nb;
   u.g = find_group(s, groups, b);
   const int j = b - s.first[u.g];
-  u.row0 = s.start[u.g] + j * ROWS;
-  u.valid = s.count[u.g] - j * ROWS;
+  u.row0 = s.start[u.g] + j * kWRows;
+  u.valid = s.count[u.g] - j * kWRows;
   return u;
 }
 
@@ -544,33 +551,50 @@ __device__ __forceinline__ bool epilogue_any(bool stop) {
   return any != 0;
 }
 
-template <typename OUT, bool RELU, int ROWS>
+// One product, or (FUSED) the two of a block of experts.
+struct WeightsArgs {
+  Fp8GemmArgs p[2];
+  int32_t* ticket;  // FUSED: next unit
+  int32_t* done;    // FUSED: per 128-row block, finished units of the first product
+};
+struct WeightsMaps {
+  CUtensorMap a[2], w[2], sa[2], sw[2];
+};
+
+__device__ __forceinline__ int ld_acquire_gpu(const int32_t* p) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
+// T: the 16-bit output type (of the second product when FUSED, whose first
+// writes e4m3).
+template <typename T, bool FUSED>
 __global__ void __launch_bounds__(kThreads, 1)
-    fp8_weights_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
-                       const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSW,
-                       Fp8GemmArgs args) {
-  using Cfg = SwapCfg<ROWS>;
-  constexpr bool OUT8 = sizeof(OUT) == 1;
-  constexpr int kStages = Cfg::kStages;
+    fp8_weights_kernel(const __grid_constant__ WeightsMaps maps, const __grid_constant__ WeightsArgs args) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ Groups grp;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sW = smem;
-  uint8_t* sA = sW + kStages * Cfg::kW;
-  uint8_t* sSf = sA + kStages * Cfg::kA;
-  float* sStg = reinterpret_cast<float*>(sSf + kStages * Cfg::kSf);
-  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sStg) + Cfg::kStg);
-  uint64_t* empty = full + kStages;
-  uint64_t* acc_full = empty + kStages;
+  uint8_t* sA = sW + kWStages * kWW;
+  uint8_t* sSf = sA + kWStages * kWA;
+  float* sStg = reinterpret_cast<float*>(sSf + kWStages * kWSf);
+  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sStg) + kWStg);
+  uint64_t* empty = full + kWStages;
+  uint64_t* acc_full = empty + kWStages;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* sf_done = acc_empty + 2;
-  uint64_t* drain = sf_done + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* q_full = sf_done + 2;
+  uint64_t* q_empty = q_full + kWQueue;
+  uint64_t* drain = q_empty + kWQueue;
+  volatile int* queue = reinterpret_cast<volatile int*>(drain + 1);  // [kWQueue], -1: no more units
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1) + kWQueue;
   volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = warp_id(), lane = lane_id();
+  int* err = args.p[0].err;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kWStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -579,150 +603,224 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&acc_empty[i], kEpi);
       mbar_init(&sf_done[i], 1);
     }
+    for (int i = 0; i < kWQueue; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1 + kEpi);
+    }
     mbar_init(drain, 1);
     *abort_s = 0;
     fence_barrier_init();
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmW);
-    tma_prefetch_desc(&tmSA);
-    tma_prefetch_desc(&tmSW);
+    for (int i = 0; i < (FUSED ? 2 : 1); ++i) {
+      tma_prefetch_desc(&maps.a[i]);
+      tma_prefetch_desc(&maps.w[i]);
+      tma_prefetch_desc(&maps.sa[i]);
+      tma_prefetch_desc(&maps.sw[i]);
+    }
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, Cfg::kTmemCols);
+    tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (!args.early) {
-    pdl_wait();
-    pdl_trigger();
-  }
-  load_groups(args, ROWS, grp);
+  pdl_wait();
+  pdl_trigger();
+  load_groups(args.p[0], kWRows, grp);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int num_n = (args.n + 127) / 128;
-  const int total = grp.first[args.groups] * num_n;
-  const int num_kb = (args.k + kBK - 1) / kBK;
+  const int groups = args.p[0].groups;
+  const int blocks = grp.first[groups];
+  const int num_n0 = (args.p[0].n + 127) / 128;
+  const int num_n1 = FUSED ? (args.p[1].n + 127) / 128 : 0;
+  const int total0 = blocks * num_n0;
+  const int total = total0 + blocks * num_n1;
+  // Unit t: product, 128-row block, column tile.
+  auto decode = [&](int t, int& ph, int& b) {
+    ph = FUSED && t >= total0 ? 1 : 0;
+    const int r = t - (ph ? total0 : 0), n = ph ? num_n1 : num_n0;
+    b = r / n;
+    return weights_unit(grp, groups, b, r - b * n);
+  };
+  // The consumers' next unit (-1: none): drawn by the producer when FUSED.
+  int taken = 0;
+  auto next_unit = [&](int t) -> int {
+    if constexpr (!FUSED) {
+      t = taken++ ? t + static_cast<int>(gridDim.x) : static_cast<int>(blockIdx.x);
+      return t < total ? t : -1;
+    } else {
+      const int s = taken % kWQueue;
+      if (!mbar_wait(&q_full[s], (taken / kWQueue) & 1, err, kErrTimeoutFull)) {
+        *abort_s = 1;
+        return -1;
+      }
+      t = queue[s];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_empty[s]);
+      ++taken;
+      return t;
+    }
+  };
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
     int stage = 0;
     uint32_t phase = 0, armed = 0, armed_parity = 0;
+    int drawn = 0, ahead = 0;
+    if (FUSED) {
+      if (lane == 0) ahead = atomicAdd(args.ticket, 1);
+      ahead = __shfl_sync(0xffffffffu, ahead, 0);
+    } else {
+      ahead = blockIdx.x;
+    }
     bool ok = true;
-    auto load_rows = [&](int st, int kb, const Unit& u, int boxes) {  // the elected lane
-      for (int i = 0; i < boxes; ++i)
-        tma_load_2d(sA + st * Cfg::kA + i * 32 * kBK, &tmA, kb * kBK, u.row0 + 32 * i, &full[st]);
-      if ((kb & 3) == 0) tma_load_3d(sSf + st * Cfg::kSf + kScaleTile, &tmSA, 0, kb >> 2, u.row0 >> 7, &full[st]);
-    };
-    // With `early`, the first unit's first stages get their weights before
-    // the wait for the previous kernel and their rows after it.
-    bool waited = !args.early;
-    int deferred = 0;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      const Unit u = weights_unit<ROWS>(grp, args.groups, t, num_n);
-      const int boxes = (min(u.valid, ROWS) + 31) / 32;
+    while (ok) {
+      const int t = ahead < total ? ahead : -1;
+      if (FUSED) {
+        const int s = drawn % kWQueue;
+        if (!mbar_wait(&q_empty[s], ((drawn / kWQueue) & 1) ^ 1, err, kErrTimeoutEmpty) || *abort_s) {
+          *abort_s = 1;
+          break;
+        }
+        if (lane == 0) {
+          queue[s] = t;
+          mbar_arrive(&q_full[s]);  // releases the store
+        }
+        __syncwarp();
+        ++drawn;
+      }
+      if (t < 0) break;
+      int ticket = 0;
+      if (FUSED && lane == 0) ticket = atomicAdd(args.ticket, 1);  // answered while this unit loads
+      int ph, b;
+      const Unit u = decode(t, ph, b);
+      const int num_kb = ((ph ? args.p[1].k : args.p[0].k) + kBK - 1) / kBK;
+      const int num_n = ph ? num_n1 : num_n0;
+      const int boxes = (min(u.valid, kWRows) + 31) / 32;
+      const CUtensorMap *mA = &maps.a[ph], *mW = &maps.w[ph], *mSA = &maps.sa[ph], *mSW = &maps.sw[ph];
+      auto load_rows = [&](int st, int kb) {  // the elected lane
+        for (int i = 0; i < boxes; ++i)
+          tma_load_2d(sA + st * kWA + i * 32 * kBK, mA, kb * kBK, u.row0 + 32 * i, &full[st]);
+        if ((kb & 3) == 0) tma_load_3d(sSf + st * kWSf + kScaleTile, mSA, 0, kb >> 2, u.row0 >> 7, &full[st]);
+      };
+      // Whether the unit's rows have been written; those of the second
+      // product come from the first. Its proxy fence orders the TMA loads
+      // behind the counter's acquire.
+      bool ready = !FUSED || ph == 0;
+      auto poll = [&]() {
+        int v = lane == 0 ? ld_acquire_gpu(args.done + b) : 0;
+        v = __shfl_sync(0xffffffffu, v, 0);
+        if (v >= num_n0) {
+          asm volatile("fence.proxy.async.global;" ::: "memory");
+          ready = true;
+        }
+      };
+      int waiting = 0, first_stage = stage;  // stages that have their weights only
       for (int kb = 0; kb < num_kb; ++kb) {
-        if (!mbar_wait(&empty[stage], phase ^ 1, args.err, kErrTimeoutEmpty) || *abort_s) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, err, kErrTimeoutEmpty) || *abort_s) {
           *abort_s = 1;
           ok = false;
           break;
         }
         if (elect_one()) {
           const bool sf = (kb & 3) == 0;
-          mbar_arrive_expect_tx(&full[stage], Cfg::kW + boxes * 32 * kBK + (sf ? Cfg::kSf : 0));
-          tma_load_3d(sW + stage * Cfg::kW, &tmW, kb * kBK, u.nb * 128, u.g, &full[stage]);
-          if (sf) tma_load_3d(sSf + stage * Cfg::kSf, &tmSW, 0, kb >> 2, u.g * num_n + u.nb, &full[stage]);
-          if (waited) load_rows(stage, kb, u, boxes);
+          mbar_arrive_expect_tx(&full[stage], kWW + boxes * 32 * kBK + (sf ? kWSf : 0));
+          tma_load_3d(sW + stage * kWW, mW, kb * kBK, u.nb * 128, u.g, &full[stage]);
+          if (sf) tma_load_3d(sSf + stage * kWSf, mSW, 0, kb >> 2, u.g * num_n + u.nb, &full[stage]);
+          if (ready) load_rows(stage, kb);
         }
-        if (!waited && (++deferred == kStages || deferred == num_kb)) {
-          pdl_wait();
-          pdl_trigger();
-          waited = true;
-          if (elect_one())
-            for (int j = 0; j < deferred; ++j) load_rows(j, j, u, boxes);
+        __syncwarp();
+        if (FUSED && !ready) {
+          ++waiting;
+          poll();
+          if (!ready && (waiting == kWStages || waiting == num_kb)) {
+            const uint64_t t0 = globaltimer_ns();
+            while (!ready) {
+              __nanosleep(64);
+              poll();
+              if (!ready && (globaltimer_ns() - t0 > AGM_WAIT_LIMIT_NS || *abort_s)) {
+                if (lane == 0) raise_error(err, kErrTimeoutFull);
+                *abort_s = 1;
+                break;
+              }
+              __syncwarp();
+            }
+            // On time-out the rows are loaded all the same, so that every armed stage completes.
+            ok = ready;
+          }
+          if (ready || !ok) {
+            if (elect_one())
+              for (int j = 0; j < waiting; ++j) load_rows((first_stage + j) % kWStages, j);
+            __syncwarp();
+          }
         }
         armed |= 1u << stage;
         armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
-        __syncwarp();
-        if (++stage == kStages) {
+        if (++stage == kWStages) {
           stage = 0;
           phase ^= 1;
         }
+        if (!ok) break;
       }
-    }
-    if (!waited) {
-      // No unit (a unit's stages end the wait above): still order after the previous kernel.
-      pdl_wait();
-      pdl_trigger();
+      ahead = FUSED ? __shfl_sync(0xffffffffu, ticket, 0) : t + static_cast<int>(gridDim.x);
     }
     __syncwarp();
-    for (int s = 0; s < kStages; ++s)
-      if (armed & (1u << s)) mbar_wait(&full[s], (armed_parity >> s) & 1, args.err, kErrTimeoutDrain);
+    for (int s = 0; s < kWStages; ++s)
+      if (armed & (1u << s)) mbar_wait(&full[s], (armed_parity >> s) & 1, err, kErrTimeoutDrain);
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
     const uint32_t sW_addr = smem_u32(sW), sA_addr = smem_u32(sA), sSf_addr = smem_u32(sSf);
     int stage = 0, it = 0, sf_use = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x, ++it) {
-      const Unit u = weights_unit<ROWS>(grp, args.groups, t, num_n);
-      const int n_mma = (min(u.valid, ROWS) + 31) / 32 * 32;
+    for (int t = next_unit(0); t >= 0 && ok; t = next_unit(t), ++it) {
+      int ph, b;
+      const Unit u = decode(t, ph, b);
+      const int num_kb = ((ph ? args.p[1].k : args.p[0].k) + kBK - 1) / kBK;
+      const int n_mma = (min(u.valid, kWRows) + 31) / 32 * 32;
       const int acc = it & 1;
-      if (!mbar_wait(&acc_empty[acc], ((it >> 1) & 1) ^ 1, args.err, kErrTimeoutAcc) || *abort_s) {
+      if (!mbar_wait(&acc_empty[acc], ((it >> 1) & 1) ^ 1, err, kErrTimeoutAcc) || *abort_s) {
         *abort_s = 1;
         break;
       }
       tc_fence_after();
-      const uint32_t d_tmem = tmem_base + acc * ROWS;
-      uint32_t sfw = 0, sfa = 0;
+      const uint32_t d_tmem = tmem_base + acc * kWRows;
+      uint32_t sfw = 0;
       int slot = 0;
       for (int kb = 0; kb < num_kb; ++kb) {
-        if (!mbar_wait(&full[stage], phase, args.err, kErrTimeoutFull) || *abort_s) {
+        if (!mbar_wait(&full[stage], phase, err, kErrTimeoutFull) || *abort_s) {
           *abort_s = 1;
           ok = false;
           break;
         }
         if ((kb & 3) == 0) {
           slot = sf_use & 1;
-          if (sf_use >= 2 && !mbar_wait(&sf_done[slot], ((sf_use >> 1) - 1) & 1, args.err, kErrTimeoutAcc)) {
+          if (sf_use >= 2 && !mbar_wait(&sf_done[slot], ((sf_use >> 1) - 1) & 1, err, kErrTimeoutAcc)) {
             *abort_s = 1;
             ok = false;
             break;
           }
           ++sf_use;
-          sfw = tmem_base + Cfg::kSfCol + slot * 8;
-          sfa = sfw + 4;
-          // The MMA takes the scales of its 32 rows from the first of the
-          // tile's four columns (it reads scales at multiples of 4 columns
-          // only), so the words of a later 32-row group move there.
-          const int q = ROWS == 32 ? (u.row0 >> 5) & 3 : 0;
-          if (q) {
-            uint32_t* tile = reinterpret_cast<uint32_t*>(sSf + stage * Cfg::kSf + kScaleTile);
-            tile[4 * lane] = tile[4 * lane + q];
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
+          sfw = tmem_base + kWSfCol + slot * 8;
         }
         tc_fence_after();
         if (elect_one()) {
           if ((kb & 3) == 0) {
-            const uint32_t src = sSf_addr + stage * Cfg::kSf;
-            const uint32_t dst = tmem_base + Cfg::kSfCol + slot * 8;
-            tmem_copy_scales<1>(dst, smem_desc_scale(src));
-            tmem_copy_scales<1>(dst + 4, smem_desc_scale(src + kScaleTile));
+            const uint32_t src = sSf_addr + stage * kWSf;
+            tmem_copy_scales<1>(sfw, smem_desc_scale(src));
+            tmem_copy_scales<1>(sfw + 4, smem_desc_scale(src + kScaleTile));
           }
-          const uint64_t w_desc = smem_desc_k_sw128(sW_addr + stage * Cfg::kW);
-          const uint64_t a_desc = smem_desc_k_sw128(sA_addr + stage * Cfg::kA);
+          const uint64_t w_desc = smem_desc_k_sw128(sW_addr + stage * kWW);
+          const uint64_t a_desc = smem_desc_k_sw128(sA_addr + stage * kWA);
           const uint32_t idesc = idesc_mxf8(128, n_mma, kb & 3);
 #pragma unroll
           for (int kk = 0; kk < kBK / 32; ++kk)
-            umma_mxf8<1>(d_tmem, w_desc + 2 * kk, a_desc + 2 * kk, idesc, sfw, sfa, (kb > 0 || kk > 0) ? 1u : 0u);
+            umma_mxf8<1>(d_tmem, w_desc + 2 * kk, a_desc + 2 * kk, idesc, sfw, sfw + 4, (kb > 0 || kk > 0) ? 1u : 0u);
           umma_commit(&empty[stage]);
           if ((kb & 3) == 3 || kb == num_kb - 1) umma_commit(&sf_done[slot]);
           if (kb == num_kb - 1) umma_commit(&acc_full[acc]);
         }
         __syncwarp();
-        if (++stage == kStages) {
+        if (++stage == kWStages) {
           stage = 0;
           phase ^= 1;
         }
@@ -730,7 +828,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (elect_one()) umma_commit(drain);
     __syncwarp();
-    mbar_wait(drain, 0, args.err, kErrTimeoutDrain);
+    mbar_wait(drain, 0, err, kErrTimeoutDrain);
   } else {
     // ---------------- Epilogue (warps 2..9) ----------------
     // The accumulator has an output column n per lane and a row per column:
@@ -739,39 +837,44 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int ew = warp - 2;
     const int quarter = warp & 3;
     const int half = ew >> 2;
-    const int out_k4 = scale_k4(args.n);
     int it = 0;
-    for (int t = blockIdx.x; t < total; t += gridDim.x, ++it) {
-      const Unit u = weights_unit<ROWS>(grp, args.groups, t, num_n);
+    for (int t = next_unit(0);; t = next_unit(t), ++it) {
+      // All epilogue warps leave together: one may have met a time-out.
+      if (epilogue_any(t < 0 || *abort_s)) break;
+      int ph, b;
+      const Unit u = decode(t, ph, b);
+      const Fp8GemmArgs& g = args.p[ph];
+      const bool out8 = g.c_scales != nullptr;
       const int acc = it & 1;
       const int n0 = u.nb * 128;
-      const int live = min(u.valid, ROWS);
+      const int live = min(u.valid, kWRows);
       // Rows this unit writes: its live rows, and behind a segment's last row zeros up to the next multiple of 128.
-      const int rows = (args.zero_pad && u.valid <= ROWS) ? live + ((-(u.row0 + live)) & 127) : live;
+      const int rows = (g.zero_pad && u.valid <= kWRows) ? live + ((-(u.row0 + live)) & 127) : live;
       const int chunks = (live + 31) / 32;
-      const bool in_n = n0 + quarter * 32 + lane < args.n;
-      const float b = args.bias && in_n ? __ldg(args.bias + static_cast<int64_t>(u.g) * args.n + n0 + quarter * 32 + lane)
-                                        : 0.f;
-      const bool got = mbar_wait(&acc_full[acc], (it >> 1) & 1, args.err, kErrTimeoutAcc);
+      const int out_k4 = scale_k4(g.n);
+      const bool in_n = n0 + quarter * 32 + lane < g.n;
+      const float bias = g.bias && in_n ? __ldg(g.bias + static_cast<int64_t>(u.g) * g.n + n0 + quarter * 32 + lane) : 0.f;
+      const bool got = mbar_wait(&acc_full[acc], (it >> 1) & 1, err, kErrTimeoutAcc);
       if (!got) *abort_s = 1;
       tc_fence_after();
-      for (int ch = 0; ch * 32 < rows; ++ch) {
+      bool stop = false;
+      for (int ch = 0; ch * 32 < rows && !stop; ++ch) {
         // Also: the staged rows of the chunk before have been read.
         if (epilogue_any(!got || *abort_s)) {
-          if (lane == 0) *abort_s = 1;
-          goto done;
+          stop = true;
+          break;
         }
         if (ch < chunks) {
           uint32_t r[16];
           tmem_ld_32x32b_x16(
-              tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * ROWS + 32 * ch + 16 * half, r);
+              tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kWRows + 32 * ch + 16 * half, r);
           tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float v = __uint_as_float(r[i]) + b;
-            if (RELU) v = relu_keep_nan(v);
+            float v = __uint_as_float(r[i]) + bias;
+            if (g.relu) v = relu_keep_nan(v);
             const bool ok_row = 32 * ch + 16 * half + i < live;
-            sStg[(16 * half + i) * Cfg::kStgLd + quarter * 32 + lane] = ok_row && in_n ? v : 0.f;
+            sStg[(16 * half + i) * kWStgLd + quarter * 32 + lane] = ok_row && in_n ? v : 0.f;
           }
           if (ch == chunks - 1) {
             tc_fence_before();
@@ -780,7 +883,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sStg[(16 * half + i) * Cfg::kStgLd + quarter * 32 + lane] = 0.f;
+          for (int i = 0; i < 16; ++i) sStg[(16 * half + i) * kWStgLd + quarter * 32 + lane] = 0.f;
         }
         named_bar_sync(1, 32 * kEpi);
 #pragma unroll
@@ -788,33 +891,41 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int rr = ew * 4 + i;
           if (32 * ch + rr >= rows) continue;
           const int64_t row = static_cast<int64_t>(u.row0) + 32 * ch + rr;
-          const float4 v = *reinterpret_cast<const float4*>(&sStg[rr * Cfg::kStgLd + 4 * lane]);
+          const float4 v = *reinterpret_cast<const float4*>(&sStg[rr * kWStgLd + 4 * lane]);
           const int n = n0 + 4 * lane;
-          if constexpr (OUT8) {
+          if (out8) {
             float m = fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w)));
             m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));  // non-negative floats order as ints
             const uint32_t byte = scale_byte(m);
             const float inv = inv_scale(byte);
-            if (n < args.n)
-              *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(args.c) + row * args.n + n) =
+            if (n < g.n)
+              *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(g.c) + row * g.n + n) =
                   pack_e4m3x4(inf_to_nan(v.x) * inv, inf_to_nan(v.y) * inv, inf_to_nan(v.z) * inv, inf_to_nan(v.w) * inv);
             if (lane == 0)
-              static_cast<uint8_t*>(args.c_scales)[scale_word_offset(row, u.nb >> 2, out_k4) + (u.nb & 3)] =
+              static_cast<uint8_t*>(g.c_scales)[scale_word_offset(row, u.nb >> 2, out_k4) + (u.nb & 3)] =
                   static_cast<uint8_t>(byte);
-          } else if (n < args.n) {
-            *reinterpret_cast<uint2*>(static_cast<OUT*>(args.c) + row * args.n + n) =
-                make_uint2(pack2<OUT>(v.x, v.y), pack2<OUT>(v.z, v.w));
+          } else if (n < g.n) {
+            *reinterpret_cast<uint2*>(static_cast<T*>(g.c) + row * g.n + n) =
+                make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
           }
+        }
+      }
+      if (stop) break;
+      if (FUSED && ph == 0) {
+        // The block's rows have one more column tile: publish it.
+        named_bar_sync(1, 32 * kEpi);
+        if (threadIdx.x == 64) {
+          __threadfence();
+          atomicAdd(args.done + b, 1);
         }
       }
     }
   }
-done:
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    tmem_dealloc(tmem_base, 512);
   }
 }
 
@@ -868,41 +979,58 @@ cudaError_t launch_rows(const Fp8GemmArgs& args, int num_sms, cudaStream_t strea
                        tmSB, tmA32, args);
 }
 
-template <typename OUT, bool RELU, int ROWS>
+template <typename T>
 cudaError_t launch_weights(const Fp8GemmArgs& args, int num_sms, cudaStream_t stream) {
-  CUtensorMap tmA, tmW, tmSA, tmSW;
-  if (!encode_operands(args, 1, &tmA, &tmW, &tmSA, &tmSW)) return cudaErrorInvalidValue;
-  const int smem = SwapCfg<ROWS>::kSmem;
-  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(fp8_weights_kernel<OUT, RELU, ROWS>), smem);
+  WeightsMaps maps = {};
+  if (!encode_operands(args, 1, &maps.a[0], &maps.w[0], &maps.sa[0], &maps.sw[0])) return cudaErrorInvalidValue;
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(fp8_weights_kernel<T, false>), kWSmem);
   if (e != cudaSuccess) return e;
-  const int64_t units = (args.live_rows / ROWS + args.groups) * static_cast<int64_t>((args.n + 127) / 128);
+  WeightsArgs wa = {};
+  wa.p[0] = args;
+  const int64_t units = (args.live_rows / kWRows + args.groups) * static_cast<int64_t>((args.n + 127) / 128);
   const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(num_sms, units)));
-  return launch_kernel(fp8_weights_kernel<OUT, RELU, ROWS>, dim3(grid), dim3(kThreads), smem, stream, tmA, tmW, tmSA,
-                       tmSW, args);
+  return launch_kernel(fp8_weights_kernel<T, false>, dim3(grid), dim3(kThreads), kWSmem, stream, maps, wa);
 }
 
-template <typename OUT, bool RELU>
-cudaError_t launch_mode(const Fp8GemmArgs& args, int mode, int num_sms, cudaStream_t stream) {
-  if (mode == AGM_FP8_ROWS) return launch_rows<OUT, RELU>(args, num_sms, stream);
-  // Up to 32 rows per group on average: blocks of 32 rows and a deeper ring.
-  if (args.live_rows <= 32 * static_cast<int64_t>(args.groups)) return launch_weights<OUT, RELU, 32>(args, num_sms, stream);
-  return launch_weights<OUT, RELU, 128>(args, num_sms, stream);
+template <typename T>
+cudaError_t launch_both(const Fp8GemmArgs& first, const Fp8GemmArgs& second, int32_t* ticket, int32_t* done, int num_sms,
+                        cudaStream_t stream) {
+  WeightsMaps maps;
+  if (!encode_operands(first, 1, &maps.a[0], &maps.w[0], &maps.sa[0], &maps.sw[0]) ||
+      !encode_operands(second, 1, &maps.a[1], &maps.w[1], &maps.sa[1], &maps.sw[1]))
+    return cudaErrorInvalidValue;
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(fp8_weights_kernel<T, true>), kWSmem);
+  if (e != cudaSuccess) return e;
+  const WeightsArgs wa{{first, second}, ticket, done};
+  return launch_kernel(fp8_weights_kernel<T, true>, dim3(num_sms), dim3(kThreads), kWSmem, stream, maps, wa);
 }
 
 template <typename OUT>
-cudaError_t launch_out(const Fp8GemmArgs& args, int mode, int num_sms, cudaStream_t stream) {
-  return args.relu ? launch_mode<OUT, true>(args, mode, num_sms, stream)
-                   : launch_mode<OUT, false>(args, mode, num_sms, stream);
+cudaError_t launch_rows_relu(const Fp8GemmArgs& args, int num_sms, cudaStream_t stream) {
+  return args.relu ? launch_rows<OUT, true>(args, num_sms, stream) : launch_rows<OUT, false>(args, num_sms, stream);
 }
 
 }  // namespace
 
+// The rows kernel fills its 256-row tiles from about 96 rows per group on (14
+// groups, 3200 -> 1280: 16.6 us against 14.2 at 64 rows, 16.9 against 24.0 at
+// 128; 61 groups, 2000 -> 1488: 51 against 44 at 80 rows, 56 against 74 at 160).
+bool fp8_rows_pay(int64_t rows, int groups) { return rows >= 96 * static_cast<int64_t>(groups); }
+
 cudaError_t grouped_gemm_fp8(int c_dtype, const Fp8GemmArgs& args, int mode, int num_sms, cudaStream_t stream) {
-  if (mode == AGM_FP8_AUTO)
-    mode = args.live_rows >= 128 * static_cast<int64_t>(args.groups) ? AGM_FP8_ROWS : AGM_FP8_WEIGHTS;
-  if (args.c_scales) return launch_out<__nv_fp8_e4m3>(args, mode, num_sms, stream);
-  return c_dtype == AGM_BF16 ? launch_out<__nv_bfloat16>(args, mode, num_sms, stream)
-                             : launch_out<__half>(args, mode, num_sms, stream);
+  const bool rows = mode == AGM_FP8_AUTO ? fp8_rows_pay(args.live_rows, args.groups) : mode == AGM_FP8_ROWS;
+  if (!rows)
+    return c_dtype == AGM_BF16 || args.c_scales ? launch_weights<__nv_bfloat16>(args, num_sms, stream)
+                                                : launch_weights<__half>(args, num_sms, stream);
+  if (args.c_scales) return launch_rows_relu<__nv_fp8_e4m3>(args, num_sms, stream);
+  return c_dtype == AGM_BF16 ? launch_rows_relu<__nv_bfloat16>(args, num_sms, stream)
+                             : launch_rows_relu<__half>(args, num_sms, stream);
+}
+
+cudaError_t expert_products_fp8(int dtype, const Fp8GemmArgs& first, const Fp8GemmArgs& second, int32_t* ticket,
+                                int32_t* done, int num_sms, cudaStream_t stream) {
+  return dtype == AGM_BF16 ? launch_both<__nv_bfloat16>(first, second, ticket, done, num_sms, stream)
+                           : launch_both<__half>(first, second, ticket, done, num_sms, stream);
 }
 
 }  // namespace agm

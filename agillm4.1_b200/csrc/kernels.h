@@ -330,7 +330,9 @@ struct Fp8Dispatch {
   int32_t* row_of;      // [n, k], -1: nowhere
   uint8_t* q;           // [max_rows, d]
   uint8_t* scales;      // scale tiles of q
-  int* err;
+  int* err;             // cleared
+  int32_t* zero;        // [n_zero], cleared
+  int n_zero;
 };
 cudaError_t dispatch_fp8(int dtype, const Fp8Dispatch& a, int num_sms, cudaStream_t stream);
 // out[t] = (residual[t] +) sum_r weights[t, r] y[row_of[t, r]], summed in fp32.
@@ -354,14 +356,17 @@ struct Fp8GemmArgs {
   int64_t live_rows = 0;           // host bound on the sum of the counts
   bool relu = false;
   bool zero_pad = false;           // write zeros to a segment's rows behind its count
-  // seg_start, counts, w and w_scales were written at least two launches ago,
-  // each of which waited for the one before it: they may be read, and the
-  // first weights loaded, before this launch waits for the previous one.
-  bool early = false;
   void* c = nullptr;               // [a_rows, n], c_dtype, or e4m3 when c_scales is set
   void* c_scales = nullptr;
   int* err = nullptr;
 };
 cudaError_t grouped_gemm_fp8(int c_dtype, const Fp8GemmArgs& args, int mode, int num_sms, cudaStream_t stream);
+// Whether 256-row tiles pay for this many rows in these groups.
+bool fp8_rows_pay(int64_t rows, int groups);
+// Both products of a block of experts in one launch, for few rows per expert:
+// `second` reads what `first` writes, over the same segments. *ticket and
+// done[0 .. blocks of 128 rows) are zero.
+cudaError_t expert_products_fp8(int dtype, const Fp8GemmArgs& first, const Fp8GemmArgs& second, int32_t* ticket,
+                                int32_t* done, int num_sms, cudaStream_t stream);
 
 }  // namespace agm

@@ -74,6 +74,8 @@ struct ExpertsLayout {
   int32_t* counts;
   int32_t* seg_start;
   int32_t* row_of;
+  int32_t* sync;  // ticket, then finished units per 128-row block (few rows per expert)
+  int n_sync;
   uint8_t* xq;
   uint8_t* xs;
   uint8_t* hq;
@@ -91,6 +93,8 @@ ExpertsLayout carve(void* ws, int64_t n, int d, int E, int k, int H) {
   L.counts = c.take<int32_t>(sizeof(int32_t) * E);
   L.seg_start = c.take<int32_t>(sizeof(int32_t) * (E + 1));
   L.row_of = c.take<int32_t>(sizeof(int32_t) * n * k);
+  L.n_sync = agm::fp8_rows_pay(n * k, E) ? 0 : 1 + static_cast<int>(rows / 128);
+  L.sync = c.take<int32_t>(sizeof(int32_t) * L.n_sync);
   L.xq = c.take<uint8_t>(static_cast<size_t>(rows) * d);
   L.xs = c.take<uint8_t>(agm_fp8_scale_bytes(rows, d));
   L.hq = c.take<uint8_t>(static_cast<size_t>(rows) * H);
@@ -203,7 +207,8 @@ int agm_grouped_gemm_fp8(const void* a, const void* a_scales, int64_t a_rows, co
   g.k = k_in;
   g.seg_start = seg_start;
   g.counts = counts;
-  g.live_rows = a_rows;
+  // The counts are on the device: of every segment's last tile, take half as padding.
+  g.live_rows = counts ? std::max<int64_t>(1, a_rows - 64 * static_cast<int64_t>(groups)) : a_rows;
   g.relu = relu != 0;
   g.zero_pad = counts != nullptr;
   g.c = c;
@@ -257,6 +262,8 @@ int agm_moe_experts_fp8(const void* x, int dtype, int64_t n_tokens, int d, int n
   dsp.q = L.xq;
   dsp.scales = L.xs;
   dsp.err = L.err;
+  dsp.zero = L.sync;
+  dsp.n_zero = L.n_sync;
   cudaError_t e = agm::dispatch_fp8(dtype, dsp, sms, stream);  // clears the error word first
   if (e != cudaSuccess) return done(e, "dispatch_fp8");
   agm::Fp8GemmArgs g;
@@ -276,21 +283,26 @@ int agm_moe_experts_fp8(const void* x, int dtype, int64_t n_tokens, int d, int n
   g.c = L.hq;
   g.c_scales = L.hs;
   g.err = L.err;
-  e = agm::grouped_gemm_fp8(dtype, g, AGM_FP8_AUTO, sms, stream);
-  if (e != cudaSuccess) return done(e, "grouped_gemm_fp8 fc1");
-  g.a = L.hq;
-  g.a_scales = L.hs;
-  g.w = w2;
-  g.w_scales = s2;
-  g.bias = b2;
-  g.n = d;
-  g.k = hidden;
-  g.relu = false;
-  g.c = L.y;
-  g.c_scales = nullptr;
-  g.early = true;  // the segments come from the launches before FC1, the weights from before the call
-  e = agm::grouped_gemm_fp8(dtype, g, AGM_FP8_AUTO, sms, stream);
-  if (e != cudaSuccess) return done(e, "grouped_gemm_fp8 fc2");
+  agm::Fp8GemmArgs h = g;
+  h.a = L.hq;
+  h.a_scales = L.hs;
+  h.w = w2;
+  h.w_scales = s2;
+  h.bias = b2;
+  h.n = d;
+  h.k = hidden;
+  h.relu = false;
+  h.c = L.y;
+  h.c_scales = nullptr;
+  if (L.n_sync) {
+    e = agm::expert_products_fp8(dtype, g, h, L.sync, L.sync + 1, sms, stream);
+    if (e != cudaSuccess) return done(e, "expert_products_fp8");
+  } else {
+    e = agm::grouped_gemm_fp8(dtype, g, AGM_FP8_ROWS, sms, stream);
+    if (e != cudaSuccess) return done(e, "grouped_gemm_fp8 fc1");
+    e = agm::grouped_gemm_fp8(dtype, h, AGM_FP8_ROWS, sms, stream);
+    if (e != cudaSuccess) return done(e, "grouped_gemm_fp8 fc2");
+  }
   return done(agm::combine_weighted(dtype, L.y, L.row_of, weights, n_tokens, d, top_k, residual, out, sms, stream),
               "combine_weighted");
 }
