@@ -35,8 +35,8 @@
 //   12 for k = 8) go to a list in index order, where each finds its rank by
 //   counting. Where keys are too close to be told apart, those of the list,
 //   or the two that make a group's score, are formed again in fp64. Only rows
-//   with NaN, +inf under softmax, or more than 32 keys at the border go to
-//   the other kernel's selection, one by one.
+//   with more than 32 keys at the border go through the other kernel's code,
+//   one by one.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
@@ -216,92 +216,92 @@ __device__ __forceinline__ bool select_experts(const float (&l)[V], const RouteA
   return near;
 }
 
+// Routes the warp's 32 / L tokens t0, t0 + 1, ...
 template <typename T, int L, int V>
-__global__ void __launch_bounds__(kRouteThreads)
-    route_kernel(const T* __restrict__ logits, RouteArgs a, int32_t* __restrict__ idx, float* __restrict__ weights) {
+__device__ __forceinline__ void route_tokens(const T* __restrict__ logits, const RouteArgs& a, int64_t t0,
+                                             int32_t* __restrict__ idx, float* __restrict__ weights) {
   constexpr int KS = L == 32 ? 1 : AGM_ROUTE_MAX_TOPK / 8;  // L = 4 serves at most 16 experts
-  constexpr int TOK = 32 / L;
-  pdl_wait();
-  pdl_trigger();
   const int lane = lane_id(), sub = lane & (L - 1);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x / 32) * TOK;
-  for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + warp_id()) * TOK; t0 < a.n; t0 += step) {
-    const int64_t t = t0 + lane / L;
-    const bool live = t < a.n;
-    const T* row = logits + (live ? t : t0) * a.n_experts;
-    float l[V];
-    bool bad = false;
+  const int64_t t = t0 + lane / L;
+  const bool live = t < a.n;
+  const T* row = logits + (live ? t : t0) * a.n_experts;
+  float l[V];
+  bool bad = false;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int e = sub + L * j;
-      l[j] = e < a.n_experts ? Traits<T>::to_f(row[e]) : kNegInf;
-      bad |= l[j] != l[j] || (a.score == AGM_ROUTE_SOFTMAX && l[j] == INFINITY);
-    }
+  for (int j = 0; j < V; ++j) {
+    const int e = sub + L * j;
+    l[j] = e < a.n_experts ? Traits<T>::to_f(row[e]) : kNegInf;
+    bad |= l[j] != l[j] || (a.score == AGM_ROUTE_SOFTMAX && l[j] == INFINITY);
+  }
 #pragma unroll
-    for (int o = L / 2; o; o >>= 1) bad |= __shfl_xor_sync(0xffffffffu, static_cast<int>(bad), o) != 0;
-    int sel[KS];
-    const bool near = select_experts<float, L, V, KS>(l, a, sub, sel);
-    if (__any_sync(0xffffffffu, near)) {
-      int again[KS];
-      select_experts<double, L, V, KS>(l, a, sub, again);
+  for (int o = L / 2; o; o >>= 1) bad |= __shfl_xor_sync(0xffffffffu, static_cast<int>(bad), o) != 0;
+  int sel[KS];
+  const bool near = select_experts<float, L, V, KS>(l, a, sub, sel);
+  if (__any_sync(0xffffffffu, near)) {
+    int again[KS];
+    select_experts<double, L, V, KS>(l, a, sub, again);
 #pragma unroll
-      for (int i = 0; i < KS; ++i) sel[i] = near ? again[i] : sel[i];
-    }
-    // Weights of the chosen experts, from their logits. Renormalised weights
-    // are ratios: the factor exp(m) common to all scores is left out, so that
-    // they do not underflow where every chosen score does.
-    float p[KS], total = 0.f;
-    if (!a.renormalize && a.score == AGM_ROUTE_SOFTMAX) {
-      float m = kNegInf;
+    for (int i = 0; i < KS; ++i) sel[i] = near ? again[i] : sel[i];
+  }
+  // Weights of the chosen experts, from their logits. Renormalised weights
+  // are ratios: the factor exp(m) common to all scores is left out, so that
+  // they do not underflow where every chosen score does.
+  float p[KS], total = 0.f;
+  if (!a.renormalize && a.score == AGM_ROUTE_SOFTMAX) {
+    float m = kNegInf;
 #pragma unroll
-      for (int j = 0; j < V; ++j) m = fmaxf(m, l[j]);
-      m = lanes_max<float, L>(m);
+    for (int j = 0; j < V; ++j) m = fmaxf(m, l[j]);
+    m = lanes_max<float, L>(m);
 #pragma unroll
-      for (int j = 0; j < V; ++j) total += l[j] > kNegInf ? expf(l[j] - m) : 0.f;
-      total = lanes_sum<float, L>(total);
+    for (int j = 0; j < V; ++j) total += l[j] > kNegInf ? expf(l[j] - m) : 0.f;
+    total = lanes_sum<float, L>(total);
 #pragma unroll
-      for (int i = 0; i < KS; ++i) p[i] = sel[i] >= 0 ? expf(Traits<T>::to_f(row[sel[i]]) - m) : 0.f;
-    } else {
-      float c[KS], m = kNegInf;
-#pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        c[i] = sel[i] >= 0 ? Traits<T>::to_f(row[sel[i]]) : kNegInf;
-        m = fmaxf(m, a.score == AGM_ROUTE_SIGMOID ? fminf(c[i], 0.f) : c[i]);
-      }
-      m = lanes_max<float, L>(m);
-      if (!a.renormalize) m = 0.f;
-#pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        if (a.score == AGM_ROUTE_SIGMOID)
-          p[i] = c[i] > kNegInf ? expf(fminf(c[i], 0.f) - m) / (1.f + expf(-fabsf(c[i]))) : 0.f;
-        else
-          p[i] = c[i] > kNegInf ? expf(c[i] - m) : 0.f;
-        total += p[i];
-      }
-      total = a.renormalize ? lanes_sum<float, L>(total) : 1.f;
-    }
+    for (int i = 0; i < KS; ++i) p[i] = sel[i] >= 0 ? expf(Traits<T>::to_f(row[sel[i]]) - m) : 0.f;
+  } else {
+    float c[KS], m = kNegInf;
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
-      const int r = sub + L * i;
-      if (live && r < a.k) {
-        idx[t * a.k + r] = sel[i];
-        weights[t * a.k + r] = bad ? NAN : (sel[i] >= 0 ? a.scale * (p[i] / total) : 0.f);
-      }
+      c[i] = sel[i] >= 0 ? Traits<T>::to_f(row[sel[i]]) : kNegInf;
+      m = fmaxf(m, a.score == AGM_ROUTE_SIGMOID ? fminf(c[i], 0.f) : c[i]);
+    }
+    m = lanes_max<float, L>(m);
+    if (!a.renormalize) m = 0.f;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      if (a.score == AGM_ROUTE_SIGMOID)
+        p[i] = c[i] > kNegInf ? expf(fminf(c[i], 0.f) - m) / (1.f + expf(-fabsf(c[i]))) : 0.f;
+      else
+        p[i] = c[i] > kNegInf ? expf(c[i] - m) : 0.f;
+      total += p[i];
+    }
+    total = a.renormalize ? lanes_sum<float, L>(total) : 1.f;
+  }
+#pragma unroll
+  for (int i = 0; i < KS; ++i) {
+    const int r = sub + L * i;
+    if (live && r < a.k) {
+      idx[t * a.k + r] = sel[i];
+      weights[t * a.k + r] = bad ? NAN : (sel[i] >= 0 ? a.scale * (p[i] / total) : 0.f);
     }
   }
 }
 
-// The exact selection of one token by a whole warp; slot r in lane r.
+template <typename T, int L, int V>
+__global__ void __launch_bounds__(kRouteThreads)
+    route_kernel(const T* __restrict__ logits, RouteArgs a, int32_t* __restrict__ idx, float* __restrict__ weights) {
+  constexpr int TOK = 32 / L;
+  pdl_wait();
+  pdl_trigger();
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x / 32) * TOK;
+  for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + warp_id()) * TOK; t0 < a.n; t0 += step)
+    route_tokens<T, L, V>(logits, a, t0, idx, weights);
+}
+
+// One token by a whole warp, out of line.
 template <typename T>
-__device__ __noinline__ int select_exactly(const T* __restrict__ row, const RouteArgs& a) {
-  constexpr int V = AGM_ROUTE_MAX_EXPERTS / 32;
-  const int lane = lane_id();
-  float l[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) l[j] = lane + 32 * j < a.n_experts ? Traits<T>::to_f(row[lane + 32 * j]) : kNegInf;
-  int sel[1];
-  select_experts<double, 32, V, 1>(l, a, lane, sel);
-  return sel[0];
+__device__ __noinline__ void route_one(const T* __restrict__ logits, const RouteArgs& a, int64_t t,
+                                       int32_t* __restrict__ idx, float* __restrict__ weights) {
+  route_tokens<T, 32, AGM_ROUTE_MAX_EXPERTS / 32>(logits, a, t, idx, weights);
 }
 
 // Approximate exponential (within 2^-22, relative, and 1.5 |v| 2^-24 for its
@@ -340,7 +340,7 @@ __device__ __forceinline__ void bitonic8(float (&v)[8]) {  // a bitonic sequence
 __device__ __forceinline__ int owner(int e, float inv_per) { return static_cast<int>((e + 0.5f) * inv_per); }
 
 // Score in fp64; m and t: the softmax's maximum and sum.
-__device__ __noinline__ double exact_score(float l, bool sigmoid, float m, double t) {
+__device__ __forceinline__ double exact_score(float l, bool sigmoid, float m, double t) {
   const double z = exp(sigmoid ? -static_cast<double>(l) : static_cast<double>(l) - m);
   return sigmoid ? 1.0 / (1.0 + z) : z / t;
 }
@@ -353,10 +353,11 @@ struct WideSmem {
   static constexpr int kTok = 32 / L;
   static constexpr int kLane = V + 4;  // floats between two lanes' experts: 16-byte rows, no bank conflicts
   float logit[kTok][L * kLane];
+  double exact[kTok][kWideList];       // keys formed again
   float key[kTok][kWideList];
-  double exact[kTok][kWideList];
   int id[kTok][kWideList];
-  int sel[kTok][kWideTopK];
+  float sorted[kTok][kWideTopK + 4];   // keys by rank, the first k + 1
+  int sel[kTok][kWideTopK + 4];        // their experts
 };
 
 template <typename T>
@@ -442,6 +443,10 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
   if (toks == 0) return;  // whole warps; no barrier of the CTA follows
   const uint32_t part = L == 32 ? kAll : ((1u << (L & 31)) - 1u) << (tok * L);
   const float* my_logit = &sm.logit[tok][sub * LD];
+  auto place = [&](int e) {  // of expert e among the lanes' experts
+    const int c = owner(e, inv_per);
+    return c * LD + (e - c * per);
+  };
   // 2. Keys, and per quarter of the lane's experts the two largest.
   float key[V], m = 0.f, inv_t = 0.f;
 #pragma unroll
@@ -477,8 +482,16 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
         for (int j = 0; j < SB; ++j) s[j] = fast_exp(key[b * SB + j] - m) * inv_t;
       }
       if (biased) {
+        if constexpr (SB % 4 == 0) {
 #pragma unroll
-        for (int j = 0; j < SB; ++j) s[j] += bias_s[sub * LD + b * SB + j];
+          for (int j = 0; j < SB; j += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(bias_s + sub * LD + b * SB + j);
+            s[j] += f.x, s[j + 1] += f.y, s[j + 2] += f.z, s[j + 3] += f.w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < SB; ++j) s[j] += bias_s[sub * LD + b * SB + j];
+        }
       }
 #pragma unroll
       for (int j = 0; j < SB; ++j) {
@@ -487,13 +500,22 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
         k1 = max_nan(k1, c);
         key[b * SB + j] = c;
       }
-      g2 = fmaxf(fmaxf(g2, k2), fminf(g1, k1));
-      g1 = fmaxf(g1, k1);
     } else {
 #pragma unroll
       for (int j = 0; j < SB; ++j) k1 = max_nan(k1, key[b * SB + j]);
     }
-    bad |= k1 != k1;
+    if (k1 != k1) {  // NaN among them: never chosen
+      bad = true;
+      k1 = k2 = kNegInf;
+#pragma unroll
+      for (int j = b * SB; j < (b + 1) * SB; ++j) {
+        if (!(key[j] > kNegInf)) key[j] = kNegInf;
+        k2 = fmaxf(k2, fminf(k1, key[j]));
+        k1 = fmaxf(k1, key[j]);
+      }
+    }
+    g2 = fmaxf(fmaxf(g2, k2), fminf(g1, k1));
+    g1 = fmaxf(g1, k1);
     top[b] = k1;
   }
   bool near = false, kept = true;
@@ -596,7 +618,7 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
   }
   const int total = __shfl_sync(kAll, upto, (lane & ~(L - 1)) | (L - 1));
   bad = (__ballot_sync(kAll, bad) & part) != 0;
-  bool slow = bad || total > kWideList;
+  const bool crowded = total > kWideList;
   for (int at = upto - count; hit && at < kWideList; ++at) {
     const int j = __ffs(hit) - 1;
     hit &= hit - 1;
@@ -611,43 +633,40 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
   const int len = min(total, kWideList);
   const int len4 = (len + 3) & ~3;
   if (sub < len4 - len) sm.key[tok][len + sub] = kNegInf;
-  if (sub < kWideTopK) sm.sel[tok][sub] = -1;
+  for (int i = sub; i <= kWideTopK; i += L) sm.sel[tok][i] = -1;
   __syncwarp();
-  // 5. Each finds its rank: the keys above it. Another key as close as the
-  // error of keys leaves the order open; an equal one goes by its index.
-  const float slack = biased ? error : 0.f;
+  // 5. Each finds its rank: the number of keys above it.
+  const bool live = tok < toks;
   for (int p = sub; p < len; p += L) {
     const float c = sm.key[tok][p];
-    const float close = slack * (1.f + fabsf(c));
-    const float hi = c + close, lo = c - close;
-    int above = 0, reach = 0;
+    int above = 0;
     for (int q = 0; q < len4; q += 4) {
       const float4 o = *reinterpret_cast<const float4*>(&sm.key[tok][q]);
-      above += (o.x > hi) + (o.y > hi) + (o.z > hi) + (o.w > hi);
-      reach += (o.x >= lo) + (o.y >= lo) + (o.z >= lo) + (o.w >= lo);
+      above += (o.x > c) + (o.y > c) + (o.z > c) + (o.w > c);
     }
-    if (reach != above + 1) {
-      const int ep = sm.id[tok][p], cp = owner(ep, inv_per), ap = cp * LD + ep - cp * per;
-      above = 0;
-      for (int q = 0; q < len; ++q) {
-        const float o = sm.key[tok][q];
-        above += o > c || (o == c && q < p);
-        if (biased && q != p && fabsf(o - c) <= close) {
-          // Equal logits with equal biases are equal keys.
-          const int eq = sm.id[tok][q], cq = owner(eq, inv_per), aq = cq * LD + eq - cq * per;
-          near |= !(bias_s[ap] == bias_s[aq] && sm.logit[tok][ap] == sm.logit[tok][aq]);
-        }
-      }
+    if (above <= a.k) {
+      sm.sel[tok][above] = sm.id[tok][p];
+      sm.sorted[tok][above] = c;
     }
-    if (above < a.k) sm.sel[tok][above] = sm.id[tok][p];
   }
-  if (__any_sync(kAll, near)) {
+  __syncwarp();
+  // Neighbours closer than the error of keys leave the order open; equal keys
+  // leave a rank empty.
+  if (sub < a.k && sub < len) {
+    const float c = sm.sorted[tok][sub];
+    const bool more = sub + 1 < len;
+    near = sm.sel[tok][sub] < 0 || (more && sm.sel[tok][sub + 1] < 0) ||
+           (biased && more && c - sm.sorted[tok][sub + 1] <= error * (1.f + fabsf(c)));
+  }
+  if (__any_sync(kAll, near && live)) {
     need_sum();
-    near = (__ballot_sync(kAll, near) & part) != 0;
+    near = (__ballot_sync(kAll, near) & part) != 0 && live;
+    __syncwarp();
+    // Again with exact keys (the logits, where there is no bias), equal ones by index.
     if (near)
       for (int p = sub; p < len; p += L) {
-        const int ep = sm.id[tok][p], cp = owner(ep, inv_per), ap = cp * LD + ep - cp * per;
-        sm.exact[tok][p] = exact_score(sm.logit[tok][ap], sigmoid, m, exact_t) + bias_s[ap];
+        const int e = sm.id[tok][p];
+        sm.exact[tok][p] = biased ? exact_score(sm.logit[tok][place(e)], sigmoid, m, exact_t) + a.bias[e] : sm.key[tok][p];
       }
     __syncwarp();
     if (near)
@@ -658,22 +677,11 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
         if (above < a.k) sm.sel[tok][above] = sm.id[tok][p];
       }
   }
-  const bool live = tok < toks;
-  slow = slow && live;
   __syncwarp();
-  uint32_t open = __ballot_sync(kAll, slow && sub == 0);
-  while (open) {  // tokens left to the exact selection, one at a time
-    const int k = (__ffs(open) - 1) / L;
-    open &= open - 1;
-    const int e = select_exactly<T>(logits + (t0 + k) * E, a);
-    if (lane < a.k) sm.sel[k][lane] = e;
-    __syncwarp();
-  }
   // 6. Weights.
-  const bool slot = live && sub < a.k;
+  const bool slot = live && sub < a.k && !crowded;
   const int e = slot ? sm.sel[tok][sub] : -1;
-  const int c = e >= 0 ? owner(e, inv_per) : 0;
-  const float l = e >= 0 ? sm.logit[tok][c * LD + (e - c * per)] : kNegInf;
+  const float l = e >= 0 ? sm.logit[tok][place(e)] : kNegInf;
   float p = 0.f, total_p = 1.f;
   if (a.renormalize) {
     const float own = sigmoid ? fminf(l, 0.f) : l;
@@ -689,14 +697,17 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
     bool nan_row = false;
     if (bad) {  // a NaN bias is no NaN logit
       for (int i = 0; i < E; ++i) {
-        const int ci = owner(i, inv_per);
-        const float v = sm.logit[tok][ci * LD + (i - ci * per)];
+        const float v = sm.logit[tok][place(i)];
         nan_row |= v != v || (!sigmoid && v == INFINITY);
       }
     }
     idx[(t0 + tok) * a.k + sub] = e;
     weights[(t0 + tok) * a.k + sub] = nan_row ? NAN : (e >= 0 ? a.scale * (p / total_p) : 0.f);
   }
+  // 7. Tokens with more keys at the border than the list holds, one by one.
+  // Last, so that the call keeps nothing of the above alive.
+  for (uint32_t open = __ballot_sync(kAll, crowded && live && sub == 0); open; open &= open - 1)
+    route_one<T>(logits, a, t0 + (__ffs(open) - 1) / L, idx, weights);
 }
 
 // d l from d w. With s the scores and w' the renormalised weights:
