@@ -351,6 +351,7 @@ constexpr int kWideList = 32;
 template <int L, int V>
 struct WideSmem {
   static constexpr int kTok = 32 / L;
+  static constexpr int kSlots = L < kWideTopK ? kWideTopK / L : 1;  // slots of a lane
   static constexpr int kLane = V + 4;  // floats between two lanes' experts: 16-byte rows, no bank conflicts
   float logit[kTok][L * kLane];
   double exact[kTok][kWideList];       // keys formed again
@@ -632,7 +633,7 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
   }
   const int len = min(total, kWideList);
   const int len4 = (len + 3) & ~3;
-  if (sub < len4 - len) sm.key[tok][len + sub] = kNegInf;
+  for (int i = len + sub; i < len4; i += L) sm.key[tok][i] = kNegInf;
   for (int i = sub; i <= kWideTopK; i += L) sm.sel[tok][i] = -1;
   __syncwarp();
   // 5. Each finds its rank: the number of keys above it.
@@ -640,9 +641,19 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
   for (int p = sub; p < len; p += L) {
     const float c = sm.key[tok][p];
     int above = 0;
-    for (int q = 0; q < len4; q += 4) {
-      const float4 o = *reinterpret_cast<const float4*>(&sm.key[tok][q]);
-      above += (o.x > c) + (o.y > c) + (o.z > c) + (o.w > c);
+    if constexpr (RAW) {
+      // Keys are exact: an equal one before p is above it too, o > c being o >= the float after c.
+      const float up = __int_as_float(__float_as_int(c) + (c < 0.f ? -1 : 1));
+      for (int q = 0; q < len4; q += 4) {
+        const float4 o = *reinterpret_cast<const float4*>(&sm.key[tok][q]);
+        above += (o.x >= (q < p ? c : up)) + (o.y >= (q + 1 < p ? c : up)) + (o.z >= (q + 2 < p ? c : up)) +
+                 (o.w >= (q + 3 < p ? c : up));
+      }
+    } else {
+      for (int q = 0; q < len4; q += 4) {
+        const float4 o = *reinterpret_cast<const float4*>(&sm.key[tok][q]);
+        above += (o.x > c) + (o.y > c) + (o.z > c) + (o.w > c);
+      }
     }
     if (above <= a.k) {
       sm.sel[tok][above] = sm.id[tok][p];
@@ -652,14 +663,14 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
   __syncwarp();
   // Neighbours closer than the error of keys leave the order open; equal keys
   // leave a rank empty.
-  if (sub < a.k && sub < len) {
-    const float c = sm.sorted[tok][sub];
-    const bool more = sub + 1 < len;
-    near = sm.sel[tok][sub] < 0 || (more && sm.sel[tok][sub + 1] < 0) ||
-           (biased && more && c - sm.sorted[tok][sub + 1] <= error * (1.f + fabsf(c)));
+  for (int r = sub; !RAW && r < a.k && r < len; r += L) {
+    const float c = sm.sorted[tok][r];
+    const bool more = r + 1 < len;
+    near |= sm.sel[tok][r] < 0 || (more && sm.sel[tok][r + 1] < 0) ||
+            (biased && more && c - sm.sorted[tok][r + 1] <= error * (1.f + fabsf(c)));
   }
-  if (__any_sync(kAll, near && live)) {
-    need_sum();
+  if (!RAW && __any_sync(kAll, near && live)) {
+    if (biased) need_sum();
     near = (__ballot_sync(kAll, near) & part) != 0 && live;
     __syncwarp();
     // Again with exact keys (the logits, where there is no bias), equal ones by index.
@@ -679,30 +690,51 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
   }
   __syncwarp();
   // 6. Weights.
-  const bool slot = live && sub < a.k && !crowded;
-  const int e = slot ? sm.sel[tok][sub] : -1;
-  const float l = e >= 0 ? sm.logit[tok][place(e)] : kNegInf;
-  float p = 0.f, total_p = 1.f;
+  constexpr int SLOTS = Smem::kSlots;
+  int e[SLOTS];
+  float l[SLOTS], p[SLOTS], total_p = 1.f;
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) {
+    const int r = sub + L * i;
+    e[i] = live && r < a.k ? sm.sel[tok][r] : -1;
+    l[i] = e[i] >= 0 ? sm.logit[tok][place(e[i])] : kNegInf;
+    p[i] = 0.f;
+  }
   if (a.renormalize) {
-    const float own = sigmoid ? fminf(l, 0.f) : l;
-    const float mx = lanes_max<float, L>(own);
-    if (e >= 0) p = expf(own - mx) / (sigmoid ? 1.f + expf(-fabsf(l)) : 1.f);
-    total_p = lanes_sum<float, L>(p);
+    float mx = kNegInf;
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) mx = fmaxf(mx, sigmoid ? fminf(l[i], 0.f) : l[i]);
+    mx = lanes_max<float, L>(mx);
+    total_p = 0.f;
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      if (e[i] >= 0) p[i] = expf((sigmoid ? fminf(l[i], 0.f) : l[i]) - mx) / (sigmoid ? 1.f + expf(-fabsf(l[i])) : 1.f);
+      total_p += p[i];
+    }
+    total_p = lanes_sum<float, L>(total_p);
     // A renormalised softmax does not look at the other logits: +inf among them is met here.
     bad |= !sigmoid && mx == INFINITY;
-  } else if (e >= 0) {
-    p = sigmoid ? expf(fminf(l, 0.f)) / (1.f + expf(-fabsf(l))) : expf(l - m) * inv_t;
+  } else {
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i)
+      if (e[i] >= 0) p[i] = sigmoid ? expf(fminf(l[i], 0.f)) / (1.f + expf(-fabsf(l[i]))) : expf(l[i] - m) * inv_t;
   }
-  if (slot) {
-    bool nan_row = false;
-    if (bad) {  // a NaN bias is no NaN logit
-      for (int i = 0; i < E; ++i) {
-        const float v = sm.logit[tok][place(i)];
-        nan_row |= v != v || (!sigmoid && v == INFINITY);
+  bool nan_row = false;
+  if (bad && live) {  // a NaN bias is no NaN logit
+    for (int i = 0; i < E; ++i) {
+      const float v = sm.logit[tok][place(i)];
+      nan_row |= v != v || (!sigmoid && v == INFINITY);
+    }
+  }
+  if (live && !crowded) {
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      const int r = sub + L * i;
+      if (r < a.k) {
+        idx[(t0 + tok) * a.k + r] = e[i];
+        weights[(t0 + tok) * a.k + r] = nan_row ? NAN : (e[i] >= 0 ? a.scale * (p[i] / total_p) : 0.f);
       }
     }
-    idx[(t0 + tok) * a.k + sub] = e;
-    weights[(t0 + tok) * a.k + sub] = nan_row ? NAN : (e >= 0 ? a.scale * (p / total_p) : 0.f);
   }
   // 7. Tokens with more keys at the border than the list holds, one by one.
   // Last, so that the call keeps nothing of the above alive.
@@ -710,40 +742,41 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
     route_one<T>(logits, a, t0 + (__ffs(open) - 1) / L, idx, weights);
 }
 
-// d l from d w. With s the scores and w' the renormalised weights:
-//   softmax, renormalised   dl_r = scale w'_r (dw_r - sum_j dw_j w'_j)
-//   sigmoid, renormalised   dl_r = scale w'_r (1 - s_r) (dw_r - sum_j dw_j w'_j)
-//   sigmoid                 dl_r = scale dw_r s_r (1 - s_r)
-//   softmax                 dl_e = s_e (scale dw_e - scale sum_j dw_j s_j), every e
+// d l from d w. With s the scores, w' the renormalised weights, G_e the sum of
+// scale dw over the slots that chose e and n_e their number:
+//   softmax, renormalised   dl_e = w'_e (G_e - n_e inner),           inner = sum_e w'_e G_e
+//   sigmoid, renormalised   dl_e = w'_e (1 - s_e) (G_e - n_e inner)
+//   sigmoid                 dl_e = s_e (1 - s_e) G_e
+//   softmax                 dl_e = s_e (G_e - sum_j s_j G_j)
 // All but the last are zero outside the chosen experts. An index outside
 // [0, E) is an empty slot; a repeated one adds up.
 // Lane i of L holds the experts [i V, (i + 1) V), so that whole rows move in
-// 16-byte (8-byte) units where they are aligned.
+// 16-byte (8-byte) units where they are aligned. A span as it is in memory:
 template <typename T, int V>
-__device__ __forceinline__ void load_span(const T* __restrict__ row, int e0, int E, int vec, float (&l)[V]) {
-  if (vec) {
+struct RawSpan {
+  T v[V];
+  __device__ __forceinline__ void load(const T* __restrict__ row, int e0, int E, int vec) {
+    if (vec) {
 #pragma unroll
-    for (int q = 0; q < V / 4; ++q) {
-      float v[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
-      if (e0 + 4 * q < E) {
-        if constexpr (sizeof(T) == 4) {
-          const float4 f = *reinterpret_cast<const float4*>(row + e0 + 4 * q);
-          v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(row + e0 + 4 * q);
-          const T* h = reinterpret_cast<const T*>(&u);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = Traits<T>::to_f(h[j]);
+      for (int q = 0; q < V; q += 4) {
+        if (e0 + q < E) {
+          if constexpr (sizeof(T) == 4)
+            *reinterpret_cast<float4*>(&v[q]) = *reinterpret_cast<const float4*>(row + e0 + q);
+          else
+            *reinterpret_cast<uint2*>(&v[q]) = *reinterpret_cast<const uint2*>(row + e0 + q);
         }
       }
+    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) l[4 * q + j] = v[j];
+      for (int j = 0; j < V; ++j)
+        if (e0 + j < E) v[j] = row[e0 + j];
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) l[j] = e0 + j < E ? Traits<T>::to_f(row[e0 + j]) : kNegInf;
   }
-}
+  __device__ __forceinline__ void get(float (&l)[V], int e0, int E) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) l[j] = e0 + j < E ? Traits<T>::to_f(v[j]) : kNegInf;
+  }
+};
 template <typename T, int V>
 __device__ __forceinline__ void store_span(T* __restrict__ row, int e0, int E, int vec, const float (&v)[V]) {
   if (vec) {
@@ -764,116 +797,135 @@ __device__ __forceinline__ void store_span(T* __restrict__ row, int e0, int E, i
   }
 }
 
+// The slots' values go to their experts' lanes through shared memory: of the
+// slots that chose an expert the first adds up all of them, in slot order.
+// Exponentials and reciprocals are the approximate ones, within 2^-21.
 template <typename T, int L, int V>
 __global__ void __launch_bounds__(kRouteThreads)
     route_backward_kernel(const float* __restrict__ dw, const T* __restrict__ logits, const int32_t* __restrict__ idx,
                           RouteArgs a, int vec, T* __restrict__ dl) {
   constexpr int KS = AGM_ROUTE_MAX_TOPK / L;
   constexpr int TOK = 32 / L;
+  constexpr uint32_t kAll = 0xffffffffu;
+  __shared__ __align__(16) float grad_s[kRouteThreads / 32][TOK][L * V];
+  __shared__ __align__(16) float count_s[kRouteThreads / 32][TOK][L * V];
+  const int lane = lane_id(), sub = lane & (L - 1), tok = lane / L;
+  float* mine_g = &grad_s[warp_id()][tok][sub * V];
+  float* mine_n = &count_s[warp_id()][tok][sub * V];
+#pragma unroll
+  for (int j = 0; j < V; j += 4) {
+    *reinterpret_cast<float4*>(mine_g + j) = make_float4(0.f, 0.f, 0.f, 0.f);
+    *reinterpret_cast<float4*>(mine_n + j) = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   pdl_wait();
   pdl_trigger();
-  const int lane = lane_id(), sub = lane & (L - 1);
   const bool sigmoid = a.score == AGM_ROUTE_SIGMOID;
-  const bool dense = !sigmoid && !a.renormalize;
   const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x / 32) * TOK;
-  for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + warp_id()) * TOK; t0 < a.n; t0 += step) {
-    const int64_t t = t0 + lane / L;
-    const bool live = t < a.n;
-    const int64_t tt = live ? t : t0;
-    const T* row = logits + tt * a.n_experts;
-    float l[V], m = kNegInf, total = 0.f;
-    if (dense) {
-      load_span<T, V>(row, sub * V, a.n_experts, vec, l);
-#pragma unroll
-      for (int j = 0; j < V; ++j) m = fmaxf(m, l[j]);
-      m = lanes_max<float, L>(m);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        l[j] = l[j] != kNegInf ? expf(l[j] - m) : 0.f;  // NaN stays
-        total += l[j];
-      }
-      total = lanes_sum<float, L>(total);
-    }
-    const float inv_total = total > 0.f ? 1.f / total : total;  // 0 for a row of -inf; NaN stays
-    int id[KS];
-    float c[KS], g[KS], p[KS], mc = kNegInf;
+  int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + warp_id()) * TOK;
+  // The next tokens' values are in flight while these are worked on.
+  RawSpan<T, V> raw;
+  int next_id[KS];
+  float next_g[KS];
+  auto fetch = [&](int64_t first) {
+    if (first >= a.n) return;
+    const int64_t tt = min(first + tok, a.n - 1);
+    raw.load(logits + tt * a.n_experts, sub * V, a.n_experts, vec);
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
       const int r = sub + L * i;
-      id[i] = -1;
-      c[i] = kNegInf;
-      g[i] = p[i] = 0.f;
-      if (L * i < a.k) {
-        id[i] = r < a.k ? idx[tt * a.k + r] : -1;
-        if (id[i] >= a.n_experts) id[i] = -1;
-        if (id[i] >= 0) {
-          c[i] = Traits<T>::to_f(row[id[i]]);
-          g[i] = a.scale * dw[tt * a.k + r];
-        }
-        mc = fmaxf(mc, sigmoid ? fminf(c[i], 0.f) : c[i]);
-      }
+      next_id[i] = r < a.k ? idx[tt * a.k + r] : -1;
+      next_g[i] = r < a.k ? dw[tt * a.k + r] : 0.f;
     }
-    if (a.renormalize) mc = lanes_max<float, L>(mc);
-    float sum = 0.f, inner = 0.f;
+  };
+  fetch(t0);
+  for (; t0 < a.n; t0 += step) {
+    const int64_t t = t0 + tok;
+    const bool live = t < a.n;
+    float l[V];
+    raw.get(l, sub * V, a.n_experts);
+    int id[KS];
+    float g[KS];
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
-      if (L * i < a.k && id[i] >= 0 && c[i] != kNegInf) {
-        if (dense)
-          p[i] = expf(c[i] - m) * inv_total;
-        else if (sigmoid)
-          p[i] = expf(fminf(c[i], 0.f) - (a.renormalize ? mc : 0.f)) / (1.f + expf(-fabsf(c[i])));
-        else
-          p[i] = expf(c[i] - mc);
-        sum += p[i];
-      }
+      id[i] = next_id[i] < a.n_experts ? next_id[i] : -1;
+      g[i] = id[i] >= 0 ? a.scale * next_g[i] : 0.f;
     }
-    if (a.renormalize) {
-      sum = lanes_sum<float, L>(sum);
-      const float inv_sum = sum != 0.f ? 1.f / sum : 0.f;
-#pragma unroll
-      for (int i = 0; i < KS; ++i) p[i] *= inv_sum;
-    }
-    if (a.renormalize || dense) {
-#pragma unroll
-      for (int i = 0; i < KS; ++i) inner += g[i] * p[i];
-      inner = lanes_sum<float, L>(inner);
-    }
-    float out[V];
-    const float spread = dense ? -inner * inv_total : 0.f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = dense ? spread * l[j] : 0.f;
-    // What each slot adds to its expert.
+    fetch(t0 + step);
+    __syncwarp();
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
-      if (L * i < a.k) {
-        if (dense)
-          g[i] = p[i] * g[i];
-        else if (sigmoid) {
-          const float z = expf(-fabsf(c[i]));
-          g[i] = p[i] * ((c[i] > 0.f ? z : 1.f) / (1.f + z)) * (g[i] - (a.renormalize ? inner : 0.f));
-        } else {
-          g[i] = p[i] * (g[i] - inner);
+      if (L * i >= a.k) break;
+      float sum = 0.f, n = 0.f;
+      bool first = true;
+#pragma unroll
+      for (int o = 0; o < KS; ++o) {
+        if (L * o >= a.k) break;
+        for (int q = 0; q < L && L * o + q < a.k; ++q) {
+          const int src = (lane & ~(L - 1)) | q;
+          const int oe = __shfl_sync(kAll, id[o], src);
+          const float og = __shfl_sync(kAll, g[o], src);
+          if (oe == id[i]) {
+            sum += og;
+            n += 1.f;
+            if (L * o + q < sub + L * i) first = false;
+          }
         }
-        if (id[i] < 0) g[i] = 0.f;
+      }
+      if (first && id[i] >= 0) {
+        grad_s[warp_id()][tok][id[i]] = sum;
+        count_s[warp_id()][tok][id[i]] = n;
       }
     }
-    for (int r = 0; r < a.k; ++r) {
-      int e = -1;
-      float v = 0.f;
+    __syncwarp();
+    float G[V], n[V];
 #pragma unroll
-      for (int i = 0; i < KS; ++i)
-        if (r / L == i) {
-          e = id[i];
-          v = g[i];
-        }
-      const int src = (lane & ~(L - 1)) | (r & (L - 1));
-      e = __shfl_sync(0xffffffffu, e, src);
-      v = __shfl_sync(0xffffffffu, v, src);
+    for (int j = 0; j < V; j += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(mine_g + j), y = *reinterpret_cast<const float4*>(mine_n + j);
+      G[j] = x.x, G[j + 1] = x.y, G[j + 2] = x.z, G[j + 3] = x.w;
+      n[j] = y.x, n[j + 1] = y.y, n[j + 2] = y.z, n[j + 3] = y.w;
+      *reinterpret_cast<float4*>(mine_g + j) = make_float4(0.f, 0.f, 0.f, 0.f);
+      *reinterpret_cast<float4*>(mine_n + j) = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    // Scores, up to a common factor: over all experts, or (renormalised) the chosen ones.
+    float m = kNegInf, total = 0.f, inner = 0.f;
+    if (!sigmoid || a.renormalize) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (e == sub * V + j) out[j] += v;
+        if (!a.renormalize || n[j] > 0.f) m = fmaxf(m, sigmoid ? fminf(l[j], 0.f) : l[j]);
+      m = lanes_max<float, L>(m);
     }
-    if (live) store_span<T, V>(dl + t * a.n_experts, sub * V, a.n_experts, vec, out);
+    float p[V], rest[V];  // score; 1 - score (sigmoid)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      rest[j] = 1.f;
+      if (sigmoid) {
+        const float z = fast_exp(-fabsf(l[j]));
+        const float inv = fast_rcp(1.f + z);
+        rest[j] = (l[j] > 0.f ? z : 1.f) * inv;
+        // s = e^min(l, 0) / (1 + z); renormalised, e^-m times that, which does not underflow with all of them.
+        p[j] = a.renormalize ? fast_exp(fminf(l[j], 0.f) - m) * inv : (l[j] > 0.f ? 1.f : z) * inv;
+      } else {
+        p[j] = l[j] != kNegInf ? fast_exp(l[j] - m) : 0.f;  // NaN stays
+      }
+      if (l[j] == kNegInf || (a.renormalize && !(n[j] > 0.f))) p[j] = 0.f;
+      total += a.renormalize ? n[j] * p[j] : p[j];
+      inner += p[j] * G[j];
+    }
+    if (!sigmoid || a.renormalize) {
+      total = lanes_sum<float, L>(total);
+      const float inv = total > 0.f ? 1.f / total : total;  // 0 where nothing is left; NaN stays
+      inner = lanes_sum<float, L>(inner) * inv;
+#pragma unroll
+      for (int j = 0; j < V; ++j) p[j] *= inv;
+    } else {
+      inner = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float d = G[j] - (a.renormalize ? n[j] * inner : inner);
+      l[j] = p[j] * rest[j] * d;
+    }
+    if (live) store_span<T, V>(dl + t * a.n_experts, sub * V, a.n_experts, vec, l);
   }
 }
 
@@ -914,8 +966,8 @@ bool wide_shape(const RouteArgs& a, int& lanes, int& per) {
   if (a.k > kWideTopK || a.n_experts < 32) return false;
   const bool grouped = a.top_groups < a.n_groups;
   if (grouped && (a.n_groups & (a.n_groups - 1))) return false;
-  lanes = std::max(8, grouped ? a.n_groups : 8);
-  if (a.n_experts > 32 * lanes) lanes = 16;
+  lanes = std::max(a.n_experts <= 64 ? 4 : 8, grouped ? a.n_groups : 1);
+  while (a.n_experts > 32 * lanes) lanes *= 2;
   if (grouped && a.n_experts % lanes) return false;
   per = (a.n_experts + lanes - 1) / lanes;
   return per <= 32;
@@ -927,6 +979,9 @@ cudaError_t route_t(const void* logits, const RouteArgs& a, int32_t* idx, float*
   int lanes, per;
   if (wide_shape(a, lanes, per)) {
     const T* x = static_cast<const T*>(logits);
+    if (lanes == 4)
+      return per <= 16 ? launch_wide<T, 4, 16>(x, a, per, idx, weights, stream)
+                       : launch_wide<T, 4, 32>(x, a, per, idx, weights, stream);
     if (lanes == 8)
       return per <= 8    ? launch_wide<T, 8, 8>(x, a, per, idx, weights, stream)
              : per <= 16 ? launch_wide<T, 8, 16>(x, a, per, idx, weights, stream)
