@@ -229,6 +229,13 @@ class _B200Forward:
     #            (costs one small device-to-host copy per backward);
     #   "zero" - zero tensors, without that copy.
     empty_expert_grad = "none"
+    # Precision of the expert products in inference:
+    #   "model" - the parameters' own dtype;
+    #   "fp8"   - e4m3 with a power-of-two scale per block of 128
+    #             (ops.moe_experts_fp8), from copies of the expert weights
+    #             quantised when first used and again whenever a parameter
+    #             changes. Routing stays as it is. bf16 and fp16 modules.
+    expert_precision = "model"
 
     def _packed_weights(self, device: torch.device, dtype: torch.dtype):
         """Expert weights as contiguous [E, ...] device tensors, with the
@@ -297,6 +304,48 @@ class _B200Forward:
             csh = None if sh is None else tuple(ops.cast_f32(t, compute_dtype) for t in sh)
         self._b200_cast = (key, (cast, csh))
         return cast, csh
+
+    # ---- 8-bit experts ----
+    def _fp8_weights(self, device: torch.device, dtype: torch.dtype):
+        """((w1, b1, w2, b2), shared [(w1, b1, w2, b2), ...]): the experts as
+        FP8Tensors with fp32 biases, made again whenever a parameter changes."""
+        w1, b1, w2, b2, sh = self._packed_weights(device, dtype)
+        key = (device, dtype) + tuple((p.data_ptr(), p._version) for p in self._expert_params())
+        cache = getattr(self, "_b200_fp8", None)
+        if cache is not None and cache[0] == key:
+            return cache[1]
+        with torch.no_grad():
+            def quantise(v1, c1, v2, c2):
+                return ops.quantize_fp8_weight(v1), c1.float(), ops.quantize_fp8_weight(v2), c2.float()
+
+            shared = []
+            if sh is not None:
+                shared = [quantise(*(t[s:s + 1].contiguous() for t in sh)) for s in range(sh[0].shape[0])]
+            pack = (quantise(w1, b1, w2, b2), shared)
+        self._b200_fp8 = (key, pack)
+        return pack
+
+    def _forward_fp8(self, flat: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.Tensor:
+        """The inference forward with 8-bit experts: the block's own router,
+        then ops.moe_experts_fp8. Shared experts run as dense 8-bit products
+        and enter the weighted sum with the residual."""
+        wr = self.router.weight
+        if flat.dtype not in (torch.bfloat16, torch.float16):
+            raise MoEKernelError(f"8-bit experts take bf16 or fp16 activations, not {flat.dtype}")
+        (w1, b1, w2, b2), shared = self._fp8_weights(flat.device, flat.dtype)
+        flat = flat.contiguous()
+        with torch.no_grad():
+            logits_in = self.router(flat).float() if self.router_logits == "reference_gemm" else None
+            idx, gates, _, _ = ops.router_topk(flat, wr.detach().contiguous(), self.top_k, logits_in=logits_in)
+            add = None if residual is None else residual.contiguous()
+            if shared:
+                x8 = ops.quantize_fp8(flat)
+                for v1, c1, v2, c2 in shared:
+                    h = ops.grouped_gemm_fp8(x8, v1, c1, relu=True, out_dtype=torch.float8_e4m3fn)
+                    y = ops.grouped_gemm_fp8(h, v2, c2, out_dtype=flat.dtype)
+                    add = y if add is None else add + y
+            return ops.moe_experts_fp8(flat, idx, gates.float(), w1, b1, w2, b2, residual=add,
+                                       check_errors=self.check_device_errors)
 
     # ---- expert streaming (agillm41.py:4367-4379, 7656-7668) ----
     def _host_expert_pack(self, dtype: torch.dtype):
@@ -416,6 +465,7 @@ class _B200Forward:
             and not (torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())
                                                   or ln.weight.requires_grad))
             and not self.training and not self.expert_stream and self.router_logits == "kernel"
+            and self.expert_precision == "model"
             and flat.is_cuda and wr.is_cuda and flat.dtype == wr.dtype == ln.weight.dtype == ln.bias.dtype
             and _autocast_dtype(flat.device) is None
             and x.shape[-1] <= (1536 if flat.dtype == torch.float32 else 2048)
@@ -439,7 +489,12 @@ class _B200Forward:
             raise MoEKernelError("MoEFFN (B200) runs on CUDA tensors only; there is no CPU path")
         if res is not None and (not res.is_cuda or res.device != flat.device):
             raise MoEKernelError("the residual must be on the input's GPU")
+        if self.expert_precision not in ("model", "fp8"):
+            raise MoEKernelError(f"expert_precision must be 'model' or 'fp8', not {self.expert_precision!r}")
         if self.expert_stream:
+            if self.expert_precision == "fp8":
+                raise MoEKernelError("expert_stream keeps the experts on the host in the model's precision; 8-bit "
+                                     "experts are device-resident")
             out = self._forward_expert_stream(flat)
             return (out if res is None else res + out).reshape(orig_shape)
         wr = self.router.weight
@@ -452,6 +507,15 @@ class _B200Forward:
         params = self._expert_params()
         grad = torch.is_grad_enabled() and (flat.requires_grad or wr.requires_grad
                                             or any(p.requires_grad for p in params))
+        if self.expert_precision == "fp8":
+            if grad or amp_mode:
+                raise MoEKernelError("8-bit experts run the inference forward only: call the module under "
+                                     "torch.no_grad() and without autocast")
+            if self.router_logits not in ("kernel", "reference_gemm"):
+                raise MoEKernelError(f"router_logits must be 'kernel' or 'reference_gemm', not {self.router_logits!r}")
+            if res is not None and res.dtype != flat.dtype:
+                raise MoEKernelError(f"residual dtype {res.dtype} differs from the input dtype {flat.dtype}")
+            return self._forward_fp8(flat, res).reshape(orig_shape)
         if grad or amp_mode:
             if self.router_logits != "kernel":
                 raise MoEKernelError("training and autocast route with the router kernel's logits only")
@@ -500,6 +564,8 @@ class _B200Forward:
             return self.forward(x_host)
         if torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters()):
             raise MoEKernelError("MoEFFN (B200) implements the inference forward only; run it under torch.no_grad()")
+        if self.expert_precision != "model":
+            raise MoEKernelError("forward_host runs the experts in the model's precision only")
         wr = self.router.weight
         if not wr.is_cuda:
             raise MoEKernelError("MoEFFN (B200): move the module to a CUDA device first")

@@ -15,6 +15,12 @@ with the B200 kernels as opaque nodes:
 ``agillm_moe::grouped_gemm``           one expert Linear (+ ReLU) over the row tiles (4367-4379)
 ``agillm_moe::combine``                gate-weighted ``index_add_`` of 4428 (+ shared experts)
 ``agillm_moe::moe_forward``            the whole block, ``MoEFFN.forward`` (4389-4431)
+``agillm_moe::route_experts``          general routing of given logits (``ops.route_experts``)
+``agillm_moe::quantize_fp8``           rows -> e4m3 values and scale tiles
+``agillm_moe::quantize_fp8_weight``    weights -> e4m3 values and scale tiles
+``agillm_moe::dequantize_fp8``         and back
+``agillm_moe::grouped_gemm_fp8``       expert Linear (+ ReLU) over block-scaled rows
+``agillm_moe::moe_experts_fp8``        the routed experts with 8-bit weights
 =====================================  ==========================================================
 
 Every operator launches on the current CUDA stream and allocates its outputs
@@ -135,4 +141,89 @@ def _(x, w_router, w1, b1, w2, b2, top_k, ws1=None, sb1=None, ws2=None, sb2=None
     return torch.empty_like(x)
 
 
-__all__ = ["router_topk", "dispatch_plan", "permute", "grouped_gemm", "combine", "moe_forward"]
+@torch.library.custom_op(f"{_NS}::route_experts", mutates_args=())
+def route_experts(logits: torch.Tensor, top_k: int, score: str, bias: Optional[torch.Tensor], n_groups: int,
+                  top_groups: int, renormalize: bool, scale: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(idx int32 [N, k], weights fp32 [N, k]) of router logits [N, E]."""
+    _cuda(logits, bias)
+    return ops.route_experts(logits.contiguous(), top_k, score=score, bias=bias, n_groups=n_groups,
+                             top_groups=top_groups, renormalize=renormalize, scale=scale)
+
+
+@route_experts.register_fake
+def _(logits, top_k, score, bias, n_groups, top_groups, renormalize, scale):
+    n = logits.shape[0]
+    return logits.new_empty(n, top_k, dtype=torch.int32), logits.new_empty(n, top_k, dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{_NS}::quantize_fp8", mutates_args=())
+def quantize_fp8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows [rows, width] -> (e4m3 [rows, width], scale tiles uint8)."""
+    _cuda(x)
+    return tuple(ops.quantize_fp8(x.contiguous()))
+
+
+@quantize_fp8.register_fake
+def _(x):
+    return x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(ops._scale_shape(*x.shape), dtype=torch.uint8)
+
+
+@torch.library.custom_op(f"{_NS}::quantize_fp8_weight", mutates_args=())
+def quantize_fp8_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Weights [G, n, width] -> (e4m3 [G, n, width], scale tiles uint8)."""
+    _cuda(w)
+    return tuple(ops.quantize_fp8_weight(w.contiguous()))
+
+
+@quantize_fp8_weight.register_fake
+def _(w):
+    return (w.new_empty(w.shape, dtype=torch.float8_e4m3fn),
+            w.new_empty((w.shape[0], *ops._scale_shape(*w.shape[1:])), dtype=torch.uint8))
+
+
+@torch.library.custom_op(f"{_NS}::dequantize_fp8", mutates_args=())
+def dequantize_fp8(q: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """The values that e4m3 q and its scale tiles stand for."""
+    _cuda(q, scales)
+    return ops.dequantize_fp8(ops.FP8Tensor(q, scales), dtype)
+
+
+@dequantize_fp8.register_fake
+def _(q, scales, dtype):
+    return q.new_empty(q.shape, dtype=dtype)
+
+
+@torch.library.custom_op(f"{_NS}::grouped_gemm_fp8", mutates_args=())
+def grouped_gemm_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
+                     bias: Optional[torch.Tensor], relu: bool, seg_start: Optional[torch.Tensor],
+                     counts: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
+    """act(a @ w[g]^T + bias[g]) for the rows of every group, bf16 or fp16."""
+    _cuda(a, a_scales, w, w_scales, bias, seg_start, counts)
+    if out_dtype not in (torch.bfloat16, torch.float16):
+        raise MoEKernelError(f"out_dtype must be bfloat16 or float16, not {out_dtype}")
+    return ops.grouped_gemm_fp8(ops.FP8Tensor(a, a_scales), ops.FP8Tensor(w, w_scales), bias, relu=relu,
+                                seg_start=seg_start, counts=counts, out_dtype=out_dtype)
+
+
+@grouped_gemm_fp8.register_fake
+def _(a, a_scales, w, w_scales, bias, relu, seg_start, counts, out_dtype):
+    return a.new_empty(a.shape[0], w.shape[1], dtype=out_dtype)
+
+
+@torch.library.custom_op(f"{_NS}::moe_experts_fp8", mutates_args=())
+def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, w1: torch.Tensor, s1: torch.Tensor,
+                    b1: torch.Tensor, w2: torch.Tensor, s2: torch.Tensor, b2: torch.Tensor,
+                    residual: Optional[torch.Tensor]) -> torch.Tensor:
+    """The routed experts of a block with 8-bit weights: x [N, d] -> [N, d]."""
+    _cuda(x, idx, weights, w1, s1, b1, w2, s2, b2, residual)
+    return ops.moe_experts_fp8(x.contiguous(), idx.contiguous(), weights.contiguous(), ops.FP8Tensor(w1, s1), b1,
+                               ops.FP8Tensor(w2, s2), b2, residual=None if residual is None else residual.contiguous())
+
+
+@moe_experts_fp8.register_fake
+def _(x, idx, weights, w1, s1, b1, w2, s2, b2, residual):
+    return torch.empty_like(x)
+
+
+__all__ = ["route_experts", "quantize_fp8", "quantize_fp8_weight", "dequantize_fp8", "grouped_gemm_fp8",
+           "moe_experts_fp8", "router_topk", "dispatch_plan", "permute", "grouped_gemm", "combine", "moe_forward"]

@@ -325,6 +325,101 @@ def test_experts_repeatable_on_streams_and_in_graphs():
     assert all(torch.equal(a, b) for a, b in zip(gouts, ref))
 
 
+@pytest.mark.parametrize("n", [1, 40, 200])
+def test_small_batches_at_once(n):
+    """Both products in one launch, several such launches at a time on streams and in graphs."""
+    E, k, d, H = 14, 2, 512, 640
+    wts = make_experts(E, d, H, 1)
+    xs = [acts(n, d, 2 + i, torch.bfloat16) for i in range(4)]
+    route = [ops.route_experts(torch.randn(n, E, generator=gen(9 + i), device="cuda"), k) for i in range(4)]
+    ref = [ops.moe_experts_fp8(x, *r, *wts, check_errors=True) for x, r in zip(xs, route)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(5):
+        outs = []
+        for s, x, r in zip(streams, xs, route):
+            with torch.cuda.stream(s):
+                outs.append(ops.moe_experts_fp8(x, *r, *wts))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, ref))
+    graphs, gouts = [], []
+    for x, r in zip(xs, route):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            gouts.append(ops.moe_experts_fp8(x, *r, *wts))
+        graphs.append(g)
+    for _ in range(3):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(gouts, ref))
+
+
+@pytest.mark.parametrize("top_k,shared,residual", [(1, 0, False), (2, 0, True), (2, 2, True), (3, 1, False)])
+def test_module_with_8_bit_experts(top_k, shared, residual):
+    """MoEFFN with expert_precision "fp8" against the same routing through the definition; a changed parameter is seen."""
+    torch.manual_seed(3)
+    d, E, n, dtype = 256, 6, 150, torch.bfloat16
+    m = agillm41_b200.MoEFFN(d, mlp_mult=2, experts=E, top_k=top_k, shared_experts=shared, shared_mlp_mult=1)
+    for blk in (m.shared or []):
+        torch.nn.init.normal_(blk[2].weight, std=0.05)
+        torch.nn.init.normal_(blk[2].bias, std=0.1)
+    m = m.to(device="cuda", dtype=dtype).eval()
+    m.check_device_errors = True
+    x = acts(n, d, 4, dtype).view(3, 50, d)
+    res = acts(n, d, 5, dtype).view(3, 50, d) if residual else None
+    with torch.no_grad():
+        plain = m.forward_residual(x, res) if residual else m(x)
+        m.expert_precision = "fp8"
+        for step in range(2):
+            got = m.forward_residual(x, res) if residual else m(x)
+            idx, gates, _, _ = ops.router_topk(x.view(n, d), m.router.weight.contiguous(), top_k)
+
+            def q(mods, i):
+                return fo.read(ops.quantize_fp8_weight(torch.stack([ex[i].weight for ex in mods])))
+
+            def b(mods, i):
+                return torch.stack([ex[i].bias for ex in mods]).float()
+
+            add = None if res is None else res.view(n, d).double()
+            slack = 0.0
+            for blk in (m.shared or []):
+                y, t = fo.experts(x.view(n, d).double(), torch.zeros(n, 1, dtype=torch.int32, device="cuda"),
+                                  torch.ones(n, 1, device="cuda"), q([blk], 0), b([blk], 0), q([blk], 2), b([blk], 2), HALF[dtype])
+                # the sum with what came before is rounded to the activation type
+                add = y if add is None else add + y
+                slack = slack + t + HALF[dtype] * add.abs()
+            ref, tol = fo.experts(x.view(n, d).double(), idx, gates.float(), q(m.experts, 0), b(m.experts, 0), q(m.experts, 2),
+                                  b(m.experts, 2), HALF[dtype], add)
+            assert bool(((got.view(n, d).double() - ref).abs() <= tol + slack * (1 + HALF[dtype])).all())
+            m.experts[0][0].weight.mul_(1.5)
+            m.experts[1][2].bias.add_(0.5)
+        m.expert_precision = "model"
+        assert plain.shape == got.shape and not torch.equal(plain, got)
+    m.expert_precision = "fp8"
+    with pytest.raises(agillm41_b200.MoEKernelError):
+        m(x)                                                   # gradients wanted
+    with torch.no_grad(), pytest.raises(agillm41_b200.MoEKernelError):
+        m.expert_precision = "int3"
+        m(x)
+
+
+def test_torch_operators_match():
+    n, E, k, d, H = 70, 9, 3, 144, 272
+    x = acts(n, d, 1, torch.float16)
+    w1, b1, w2, b2 = make_experts(E, d, H, 2)
+    o = torch.ops.agillm_moe
+    idx, wgt = o.route_experts(torch.randn(n, E, generator=gen(3), device="cuda"), k, "softmax", None, 1, 1, True, 1.0)
+    y = o.moe_experts_fp8(x, idx, wgt, *w1, b1, *w2, b2, x)
+    assert torch.equal(y, ops.moe_experts_fp8(x, idx, wgt, w1, b1, w2, b2, residual=x))
+    q = o.quantize_fp8(x)
+    assert torch.equal(o.dequantize_fp8(*q, torch.float32), ops.dequantize_fp8(ops.quantize_fp8(x), torch.float32))
+    one = ops.FP8Tensor(w1.q[:1].contiguous(), w1.scales[:1].contiguous())
+    assert torch.equal(o.grouped_gemm_fp8(*q, *one, b1[:1], True, None, None, torch.float16),
+                       ops.grouped_gemm_fp8(ops.FP8Tensor(*q), one, b1[:1], relu=True, out_dtype=torch.float16))
+
+
 def test_refusals_on_the_gpu():
     E = agillm41_b200.MoEKernelError
     x = acts(8, 64, 1, torch.bfloat16)

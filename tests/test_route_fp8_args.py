@@ -121,3 +121,37 @@ def test_oracle_routing_by_hand():
     assert ro.choose(torch.full((1, 4), -math.inf), 2).tolist() == [[-1, -1]]
     w = ro.weights(l, torch.tensor([[1, 5, -1]]), "softmax", True, 2.0)
     assert torch.allclose(w, torch.tensor([[2 / (1 + math.exp(-0.5)), 2 / (1 + math.exp(0.5)), 0.0]], dtype=torch.float64))
+
+
+def test_torch_operators_shapes():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    f8 = torch.float8_e4m3fn
+    o = torch.ops.agillm_moe
+    with FakeTensorMode():
+        x = torch.empty(300, 528, dtype=torch.bfloat16, device="cuda")
+        idx, w = o.route_experts(torch.empty(300, 64, device="cuda"), 6, "sigmoid", None, 8, 4, True, 2.5)
+        assert idx.shape == w.shape == (300, 6) and idx.dtype == torch.int32 and w.dtype == torch.float32
+        q, s = o.quantize_fp8(x)
+        assert q.shape == x.shape and q.dtype == f8 and s.shape == (3, 2, 512) and s.dtype == torch.uint8
+        assert o.dequantize_fp8(q, s, torch.float32).dtype == torch.float32
+        w1, s1 = o.quantize_fp8_weight(torch.empty(64, 400, 528, device="cuda"))
+        w2, s2 = o.quantize_fp8_weight(torch.empty(64, 528, 400, device="cuda"))
+        assert s1.shape == (64, 4, 2, 512) and s2.shape == (64, 5, 1, 512)
+        y = o.grouped_gemm_fp8(q, s, w1, s1, None, True, idx[:65, 0], idx[:64, 0], torch.float16)
+        assert y.shape == (300, 400) and y.dtype == torch.float16
+        b1, b2 = torch.empty(64, 400, device="cuda"), torch.empty(64, 528, device="cuda")
+        assert o.moe_experts_fp8(x, idx, w, w1, s1, b1, w2, s2, b2, None).shape == x.shape
+
+
+def test_module_precision_is_checked():
+    import agillm41_b200
+
+    m = agillm41_b200.MoEFFN(64, mlp_mult=2, experts=4, top_k=2)
+    assert m.expert_precision == "model"
+    m.expert_precision = "fp8"
+    with pytest.raises(MoEKernelError):
+        m(torch.zeros(3, 64))                    # no CPU path
+    with pytest.raises(MoEKernelError):
+        with torch.no_grad():
+            m.forward_host(torch.zeros(3, 64))
