@@ -560,7 +560,7 @@ def _call(dev: torch.device, name: str, *args) -> None:
     """Call a C entry point on ``dev``'s current stream, whichever device is current."""
     fn = getattr(load(), name)
     stream = torch._C._cuda_getCurrentRawStream(dev.index)  # a tenth of stream_handle()'s time
-    if dev.index == torch.cuda.current_device():
+    if dev.index == torch._C._cuda_getDevice():
         rc = fn(*args, stream)
     else:
         with torch.cuda.device(dev):
@@ -570,7 +570,9 @@ def _call(dev: torch.device, name: str, *args) -> None:
 
 
 def _need(what: str, t: torch.Tensor, dtype, shape, dev: torch.device) -> None:
-    """Refuse a tensor that is not of this dtype and shape on this GPU."""
+    """Refuse a tensor that is not of this dtype and shape, contiguous, on this GPU."""
+    if t.dtype is dtype and t.device == dev and t.shape == shape and t.is_contiguous():
+        return
     if not t.is_cuda:
         raise _lib.MoEKernelError(f"{what} must be a CUDA tensor: the MoE kernels have no CPU path")
     if t.device != dev:
@@ -579,14 +581,23 @@ def _need(what: str, t: torch.Tensor, dtype, shape, dev: torch.device) -> None:
         raise _lib.MoEKernelError(f"{what} must be {dtype}, not {t.dtype}")
     if t.shape != shape:
         raise _lib.MoEKernelError(f"{what} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    raise _lib.MoEKernelError(f"{what} must be contiguous")
 
 
 def _cuda_matrix(what: str, t: torch.Tensor, dim: int = 2) -> torch.device:
+    """The GPU of a contiguous tensor of this many dimensions."""
+    if t.is_cuda and t.dim() == dim and t.is_contiguous():
+        return t.device
     if t.dim() != dim:
         raise _lib.MoEKernelError(f"{what} must have {dim} dimensions, not shape {tuple(t.shape)}")
     if not t.is_cuda:
         raise _lib.MoEKernelError(f"{what} must be a CUDA tensor: the MoE kernels have no CPU path")
-    return t.device
+    raise _lib.MoEKernelError(f"{what} must be contiguous")
+
+
+def _address(t: Optional[torch.Tensor]) -> Optional[int]:
+    """Data pointer of a checked tensor, or None."""
+    return None if t is None else t.data_ptr()
 
 
 _SCORES = {"softmax": _lib.AGM_ROUTE_SOFTMAX, "sigmoid": _lib.AGM_ROUTE_SIGMOID}
@@ -621,9 +632,9 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
         _need("bias", bias, torch.float32, (E,), dev)
     idx = torch.empty(n, top_k, dtype=torch.int32, device=dev)
     weights = torch.empty(n, top_k, dtype=torch.float32, device=dev)
-    _call(dev, "agm_route_experts", ptr(logits), dtype_code(logits.dtype), n, E, top_k, _score_code(score), ptr(bias),
-          n_groups, n_groups if top_groups is None else top_groups, int(renormalize), float(scale), ptr(idx),
-          ptr(weights))
+    _call(dev, "agm_route_experts", logits.data_ptr(), dtype_code(logits.dtype), n, E, top_k, _score_code(score),
+          _address(bias), n_groups, n_groups if top_groups is None else top_groups,
+          renormalize, scale, idx.data_ptr(), weights.data_ptr())
     return idx, weights
 
 
@@ -634,13 +645,12 @@ def route_experts_backward(dweights: torch.Tensor, logits: torch.Tensor, idx: to
     options. Slots whose index lies outside [0, E) contribute nothing."""
     dev = _cuda_matrix("logits", logits)
     n, E = logits.shape
-    _cuda_matrix("idx", idx)
-    k = idx.shape[1]
+    k = idx.shape[-1] if idx.dim() else 0
     _need("idx", idx, torch.int32, (n, k), dev)
     _need("dweights", dweights, torch.float32, (n, k), dev)
     dlogits = torch.empty_like(logits)
-    _call(dev, "agm_route_experts_backward", ptr(dweights), ptr(logits), dtype_code(logits.dtype), n, E, k, ptr(idx),
-          _score_code(score), int(renormalize), float(scale), ptr(dlogits))
+    _call(dev, "agm_route_experts_backward", dweights.data_ptr(), logits.data_ptr(), dtype_code(logits.dtype), n, E, k,
+          idx.data_ptr(), _score_code(score), renormalize, scale, dlogits.data_ptr())
     return dlogits
 
 
@@ -664,13 +674,19 @@ def _scale_shape(rows: int, width: int) -> tuple:
 
 
 def _need_fp8(what: str, t: FP8Tensor, dim: int, dev: Optional[torch.device] = None) -> torch.device:
+    """Refuse what is not an FP8Tensor of this many dimensions (on this GPU, when given); its GPU."""
     if not isinstance(t, FP8Tensor):
         raise _lib.MoEKernelError(f"{what} must be an FP8Tensor, not {type(t).__name__}")
-    dev = _cuda_matrix(f"{what}.q", t.q, dim) if dev is None else dev
-    _need(f"{what}.q", t.q, torch.float8_e4m3fn, t.q.shape, dev)
-    _cuda_matrix(f"{what}.q", t.q, dim)
-    _need(f"{what}.scales", t.scales, torch.uint8, (*t.q.shape[:-2], *_scale_shape(*t.q.shape[-2:])), dev)
-    return dev
+    q = t.q
+    own = _cuda_matrix(f"{what}.q", q, dim)
+    if dev is not None and own != dev:
+        raise _lib.MoEKernelError(f"{what} is on {own}, not on {dev}")
+    if q.dtype is not torch.float8_e4m3fn:
+        raise _lib.MoEKernelError(f"{what}.q must be {torch.float8_e4m3fn}, not {q.dtype}")
+    shape = q.shape
+    tiles = ((shape[-2] + 127) // 128, (shape[-1] + 511) // 512, 512)
+    _need(f"{what}.scales", t.scales, torch.uint8, tiles if dim == 2 else (shape[0], *tiles), own)
+    return own
 
 
 def quantize_fp8(x: torch.Tensor) -> FP8Tensor:
@@ -681,7 +697,7 @@ def quantize_fp8(x: torch.Tensor) -> FP8Tensor:
     rows, width = x.shape
     t = FP8Tensor(torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=dev),
                   torch.empty(_scale_shape(rows, width), dtype=torch.uint8, device=dev))
-    _call(dev, "agm_quantize_fp8", ptr(x), dtype_code(x.dtype), rows, width, ptr(t.q), ptr(t.scales))
+    _call(dev, "agm_quantize_fp8", x.data_ptr(), dtype_code(x.dtype), rows, width, t.q.data_ptr(), t.scales.data_ptr())
     return t
 
 
@@ -692,17 +708,19 @@ def quantize_fp8_weight(w: torch.Tensor) -> FP8Tensor:
     G, n, width = w.shape
     t = FP8Tensor(torch.empty(G, n, width, dtype=torch.float8_e4m3fn, device=dev),
                   torch.empty(G, *_scale_shape(n, width), dtype=torch.uint8, device=dev))
-    _call(dev, "agm_quantize_fp8_weight", ptr(w), dtype_code(w.dtype), G, n, width, ptr(t.q), ptr(t.scales))
+    _call(dev, "agm_quantize_fp8_weight", w.data_ptr(), dtype_code(w.dtype), G, n, width, t.q.data_ptr(),
+          t.scales.data_ptr())
     return t
 
 
 def dequantize_fp8(t: FP8Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values an :class:`FP8Tensor` stands for, rounded once to ``dtype``."""
-    dev = _need_fp8("t", t, t.q.dim() if isinstance(t, FP8Tensor) and t.q.dim() == 3 else 2)
+    dev = _need_fp8("t", t, 3 if isinstance(t, FP8Tensor) and t.q.dim() == 3 else 2)
     rows, width = t.q.shape[-2:]
     G = t.q.shape[0] if t.q.dim() == 3 else 1
     out = torch.empty(t.q.shape, dtype=dtype, device=dev)
-    _call(dev, "agm_dequantize_fp8", ptr(t.q), ptr(t.scales), G, rows, width, dtype_code(dtype), ptr(out))
+    _call(dev, "agm_dequantize_fp8", t.q.data_ptr(), t.scales.data_ptr(), G, rows, width, dtype_code(dtype),
+          out.data_ptr())
     return out
 
 
@@ -750,9 +768,9 @@ def grouped_gemm_fp8(a: FP8Tensor, w: FP8Tensor, bias: Optional[torch.Tensor] = 
         out = torch.empty(R, N, dtype=out_dtype, device=dev)
     else:
         _need("out", out, out_dtype, (R, N), dev)
-    _call(dev, "agm_grouped_gemm_fp8", ptr(a.q), ptr(a.scales), R, ptr(w.q), ptr(w.scales), ptr(bias), G, N, K,
-          ptr(seg_start), ptr(counts), int(relu), mode, ptr(out), 0 if scales is not None else dtype_code(out_dtype),
-          ptr(scales), ptr(err))
+    _call(dev, "agm_grouped_gemm_fp8", a.q.data_ptr(), a.scales.data_ptr(), R, w.q.data_ptr(), w.scales.data_ptr(),
+          _address(bias), G, N, K, _address(seg_start), _address(counts), relu, mode, out.data_ptr(),
+          0 if scales is not None else dtype_code(out_dtype), _address(scales), _address(err))
     return out if scales is None else FP8Tensor(out, scales)
 
 
@@ -779,8 +797,7 @@ def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, w
     E, H, dw = w1.q.shape
     if dw != d or w2.q.shape != (E, d, H):
         raise _lib.MoEKernelError(f"w1 {tuple(w1.q.shape)} and w2 {tuple(w2.q.shape)} do not fit x {tuple(x.shape)}")
-    _cuda_matrix("idx", idx)
-    k = idx.shape[1]
+    k = idx.shape[-1] if idx.dim() else 0
     _need("idx", idx, torch.int32, (n, k), dev)
     _need("weights", weights, torch.float32, (n, k), dev)
     _need("b1", b1, torch.float32, (E, H), dev)
@@ -790,11 +807,12 @@ def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, w
     if workspace is None:
         nbytes = int(lib.agm_moe_experts_fp8_workspace_bytes(n, d, E, k, H))
         workspace = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or workspace.dtype != torch.uint8:
-        raise _lib.MoEKernelError(f"workspace must be a uint8 tensor on {dev}")
+    elif workspace.device != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise _lib.MoEKernelError(f"workspace must be a contiguous uint8 tensor on {dev}")
     out = torch.empty_like(x)
-    _call(dev, "agm_moe_experts_fp8", ptr(x), dtype_code(x.dtype), n, d, E, k, H, ptr(idx), ptr(weights), ptr(w1.q),
-          ptr(w1.scales), ptr(b1), ptr(w2.q), ptr(w2.scales), ptr(b2), ptr(residual), ptr(out), ptr(workspace),
+    _call(dev, "agm_moe_experts_fp8", x.data_ptr(), dtype_code(x.dtype), n, d, E, k, H, idx.data_ptr(),
+          weights.data_ptr(), w1.q.data_ptr(), w1.scales.data_ptr(), b1.data_ptr(), w2.q.data_ptr(),
+          w2.scales.data_ptr(), b2.data_ptr(), _address(residual), out.data_ptr(), workspace.data_ptr(),
           workspace.numel())
     if check_errors:
         code = _lib.read_device_error(workspace[:4].view(torch.int32))
