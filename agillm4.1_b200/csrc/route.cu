@@ -216,11 +216,10 @@ __device__ __forceinline__ bool select_experts(const float (&l)[V], const RouteA
   return near;
 }
 
-// Routes the warp's 32 / L tokens t0, t0 + 1, ...
-template <typename T, int L, int V>
+// Routes the warp's 32 / L tokens t0, t0 + 1, ...; a lane holds KS of its token's slots.
+template <typename T, int L, int V, int KS>
 __device__ __forceinline__ void route_tokens(const T* __restrict__ logits, const RouteArgs& a, int64_t t0,
                                              int32_t* __restrict__ idx, float* __restrict__ weights) {
-  constexpr int KS = L == 32 ? 1 : AGM_ROUTE_MAX_TOPK / 8;  // L = 4 serves at most 16 experts
   const int lane = lane_id(), sub = lane & (L - 1);
   const int64_t t = t0 + lane / L;
   const bool live = t < a.n;
@@ -286,7 +285,7 @@ __device__ __forceinline__ void route_tokens(const T* __restrict__ logits, const
   }
 }
 
-template <typename T, int L, int V>
+template <typename T, int L, int V, int KS>
 __global__ void __launch_bounds__(kRouteThreads)
     route_kernel(const T* __restrict__ logits, RouteArgs a, int32_t* __restrict__ idx, float* __restrict__ weights) {
   constexpr int TOK = 32 / L;
@@ -294,14 +293,14 @@ __global__ void __launch_bounds__(kRouteThreads)
   pdl_trigger();
   const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x / 32) * TOK;
   for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + warp_id()) * TOK; t0 < a.n; t0 += step)
-    route_tokens<T, L, V>(logits, a, t0, idx, weights);
+    route_tokens<T, L, V, KS>(logits, a, t0, idx, weights);
 }
 
 // One token by a whole warp, out of line.
 template <typename T>
 __device__ __noinline__ void route_one(const T* __restrict__ logits, const RouteArgs& a, int64_t t,
                                        int32_t* __restrict__ idx, float* __restrict__ weights) {
-  route_tokens<T, 32, AGM_ROUTE_MAX_EXPERTS / 32>(logits, a, t, idx, weights);
+  route_tokens<T, 32, AGM_ROUTE_MAX_EXPERTS / 32, 1>(logits, a, t, idx, weights);
 }
 
 // Approximate exponential (within 2^-22, relative, and 1.5 |v| 2^-24 for its
@@ -799,12 +798,17 @@ __device__ __forceinline__ void store_span(T* __restrict__ row, int e0, int E, i
 
 // The slots' values go to their experts' lanes through shared memory: of the
 // slots that chose an expert the first adds up all of them, in slot order.
-// Exponentials and reciprocals are the approximate ones, within 2^-21.
-template <typename T, int L, int V>
+// Exponentials and reciprocals are the approximate ones, within 2^-21. A lane
+// holds KS of its token's slots: one where k <= L, which leaves registers for
+// a fourth CTA per SM and cuts the slots' code by KS^2.
+//
+// Bound by issuing instructions, not by memory: 262,144 x 64 bf16, top-6,
+// takes 43.5 us (80 MB, 1.8 TB/s; 56.5 with four slots a lane throughout),
+// 49,151 x 64 10.4 us.
+template <typename T, int L, int V, int KS>
 __global__ void __launch_bounds__(kRouteThreads)
     route_backward_kernel(const float* __restrict__ dw, const T* __restrict__ logits, const int32_t* __restrict__ idx,
                           RouteArgs a, int vec, T* __restrict__ dl) {
-  constexpr int KS = AGM_ROUTE_MAX_TOPK / L;
   constexpr int TOK = 32 / L;
   constexpr uint32_t kAll = 0xffffffffu;
   __shared__ __align__(16) float grad_s[kRouteThreads / 32][TOK][L * V];
@@ -940,9 +944,13 @@ cudaError_t by_width(int n_experts, bool grouped, Call&& call) {
   return call(integral_constant<int, 32>{}, integral_constant<int, 16>{});
 }
 
-unsigned route_grid(int64_t n, int lanes, int num_sms) {
+// At most `per_sm` CTAs per SM. The forward takes more than are resident: its
+// tokens differ (65,536 x 24, top-4: 18.5 us on 4, 15.8 on 8). The gradient
+// takes the resident 4: each CTA prefetches its next tokens (262,144 x 64, top-6:
+// 43.5 us on 4, 50.9 on 6, 44.0 on 8).
+unsigned route_grid(int64_t n, int lanes, int num_sms, int per_sm) {
   const int64_t per_cta = kRouteThreads / lanes;
-  return static_cast<unsigned>(std::min<int64_t>((n + per_cta - 1) / per_cta, static_cast<int64_t>(num_sms) * 8));
+  return static_cast<unsigned>(std::min<int64_t>((n + per_cta - 1) / per_cta, static_cast<int64_t>(num_sms) * per_sm));
 }
 
 template <typename T, int L, int V>
@@ -992,8 +1000,11 @@ cudaError_t route_t(const void* logits, const RouteArgs& a, int32_t* idx, float*
     return launch_wide<T, 32, 16>(x, a, per, idx, weights, stream);
   }
   return by_width(a.n_experts, a.top_groups < a.n_groups, [&](auto l, auto v) {
-    return launch_kernel(route_kernel<T, l.value, v.value>, dim3(route_grid(a.n, l.value, num_sms)),
-                         dim3(kRouteThreads), 0, stream, static_cast<const T*>(logits), a, idx, weights);
+    constexpr int L = l.value, V = v.value;
+    constexpr int kMost = L == 32 ? 1 : AGM_ROUTE_MAX_TOPK / 8;  // 4 lanes serve at most 16 experts
+    const auto kernel = a.k <= L ? route_kernel<T, L, V, 1> : route_kernel<T, L, V, kMost>;
+    return launch_kernel(kernel, dim3(route_grid(a.n, L, num_sms, 8)), dim3(kRouteThreads), 0, stream,
+                         static_cast<const T*>(logits), a, idx, weights);
   });
 }
 
@@ -1004,9 +1015,11 @@ cudaError_t route_backward_t(const float* dw, const void* logits, const int32_t*
   const uintptr_t at = reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(dl);
   const int vec = a.n_experts % 4 == 0 && at % (4 * sizeof(T)) == 0;
   auto launch = [&](auto l, auto v) {
-    return launch_kernel(route_backward_kernel<T, l.value, v.value>, dim3(route_grid(a.n, l.value, num_sms)),
-                         dim3(kRouteThreads), 0, stream, dw, static_cast<const T*>(logits), idx, a, vec,
-                         static_cast<T*>(dl));
+    constexpr int L = l.value, V = v.value;
+    const auto kernel = a.k <= L ? route_backward_kernel<T, L, V, 1>
+                                 : route_backward_kernel<T, L, V, AGM_ROUTE_MAX_TOPK / L>;
+    return launch_kernel(kernel, dim3(route_grid(a.n, L, num_sms, 4)), dim3(kRouteThreads), 0, stream, dw,
+                         static_cast<const T*>(logits), idx, a, vec, static_cast<T*>(dl));
   };
   const integral_constant<int, 8> v8;
   if (a.n_experts <= 32) return launch(integral_constant<int, 4>{}, v8);
