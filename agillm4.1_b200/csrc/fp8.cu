@@ -133,10 +133,14 @@ struct UnitWalk {
   }
 };
 
-constexpr int kFlight = 4;  // units of a warp in flight
+// Units of a warp in flight: one at a time, 94 M elements of bf16 took 78 us to
+// quantise and 65 us to read back; four at a time 56 and 54 us.
+constexpr int kFlight = 4;
 
 // One warp per (row, 512 columns); rows up to the next multiple of 128 get a
-// scale word only, so that whole scale tiles are defined.
+// scale word only, so that whole scale tiles are defined. Bound by memory:
+// 73,728 x 1280 bf16 in 52 us, 283 MB at 5.4 TB/s, with 61% of the issue slots
+// taken.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 3)
     quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int width, int width_k4, uint8_t* __restrict__ q,
@@ -173,7 +177,8 @@ __global__ void __launch_bounds__(kThreads, 3)
 }
 
 // One CTA per 128 x 128 block: 8 lanes hold a row of the block, 4 passes of 32
-// rows stay in registers between the maximum and the rounding.
+// rows stay in registers between the maximum and the rounding. 14 x 3200 x
+// 1280 bf16 in 31 to 35 us, 172 MB at 5.2 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     quantize_weight_kernel(const T* __restrict__ w, int n, int width, int width_k4, uint8_t* __restrict__ q,
@@ -265,7 +270,8 @@ __device__ __forceinline__ void decode_unit(const uint4& b, uint32_t word, int l
   }
 }
 
-// Rows of all groups in one sequence; a group's scale tiles start anew.
+// Rows of all groups in one sequence; a group's scale tiles start anew. 73,728
+// x 1280 to bf16 in 50 us, 5.6 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4)
     dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales, int64_t groups, int64_t rows,
@@ -324,7 +330,8 @@ __device__ __forceinline__ void padded_prefix(const int* count_s, int E, int* st
 
 // Small batches: every CTA counts all slots by itself and its warps move
 // (token, 512 columns) units, one launch in all. The unit's elements are
-// loaded before the counting, which hides their latency.
+// loaded before the counting, which hides their latency. 64 tokens, top-2 of
+// 14, width 1280: 3.7 us, a launch and three dependent reads.
 constexpr int kSmallSlots = 1024;
 template <typename T>
 __global__ void __launch_bounds__(kThreads) dispatch_small_kernel(Fp8Dispatch a, int width_k4) {
@@ -442,7 +449,10 @@ __global__ void __launch_bounds__(kThreads)
 // 3: destinations of a block's slots in slot order, then its rows. Each warp
 // ranks an eighth of the block's slots: matching lanes of 32 slots at a time,
 // on top of the counts of the warps before it. Small grids split a block's
-// rows over several CTAs, each of which ranks all its slots.
+// rows over several CTAs, each of which ranks all its slots (24 blocks: 105
+// us whole, 15.5 split; finer splits of large batches gain nothing). Bound by
+// memory and its ranking pass: 73,728 tokens x 1280 bf16, top-2, 379 MB in
+// 82 us, 4.6 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 3) dispatch_rows_kernel(Fp8Dispatch a, int width_k4, int split) {
   __shared__ int start_s[AGM_ROUTE_MAX_EXPERTS + 1];
@@ -545,7 +555,8 @@ __global__ void __launch_bounds__(kThreads, 3) dispatch_rows_kernel(Fp8Dispatch 
 // ---------------------------------------------------------------------------
 // One warp per token and P x 256 columns: a lane sums P x 8 columns over the
 // token's rows, the loads of KU rows in flight at a time. ONE: k <= KU, so
-// that only one part's sums are held at a time.
+// that only one part's sums are held at a time. Bound by memory: 73,728 tokens
+// x 1280 bf16, top-2, 567 MB in about 115 us, 4.9 TB/s.
 template <typename T, int KU, int P, bool ONE>
 __global__ void __launch_bounds__(kThreads)
     combine_weighted_kernel(const T* __restrict__ y, const int32_t* __restrict__ row_of,
@@ -619,7 +630,7 @@ __global__ void __launch_bounds__(kThreads)
 // One warp per unit, on at most `per_sm` CTAs per SM. Quantising and reading
 // back take as many as are resident at once, so that all run from start to end
 // with equal shares (94 M elements: quantise 57 us on 8 per SM, 53 us on 3;
-// read back 61 us on 8, 58 us on 4). The weighted sum's few CTAs would leave
+// read back 61 us on 8, 58 us on 4, in a loop). The weighted sum's few CTAs would leave
 // their SMs to the next launch late (73,728 tokens: 119 us on 8, 140 us on 3).
 unsigned warp_grid(int64_t units, int num_sms, int per_sm) {
   return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((units + kWarps - 1) / kWarps,

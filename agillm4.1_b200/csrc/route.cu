@@ -36,7 +36,13 @@
 //   counting. Where keys are too close to be told apart, those of the list,
 //   or the two that make a group's score, are formed again in fp64. Only rows
 //   with more than 32 keys at the border go through the other kernel's code,
-//   one by one.
+//   one by one. That case now takes 41 us: 71 MB at 1.7 TB/s, still bound by
+//   issuing (58% of the slots at 24 warps per SM). Two CTAs per SM with 128
+//   registers took 45 us, 16 lanes a token 48, 64 registers with the keys
+//   written over the logits 47. 262,144 x 64 bf16, top-6: 47 us.
+//
+// Few tokens (64 x 14: 2.3 us on the device) cost a launch and one pass's
+// latency.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
