@@ -40,6 +40,7 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from ._lib import MoEKernelError
@@ -196,6 +197,7 @@ class _RouteNode(torch.autograd.Function):
         return idx, weights
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, _, dweights):
         logits, idx = ctx.saved_tensors
         return (ops.route_experts_backward(dweights.contiguous(), logits, idx, **ctx.options),) + (None,) * 7
@@ -234,7 +236,9 @@ class _B200Forward:
     #   "fp8"   - e4m3 with a power-of-two scale per block of 128
     #             (ops.moe_experts_fp8), from copies of the expert weights
     #             quantised when first used and again whenever a parameter
-    #             changes. Routing stays as it is. bf16 and fp16 modules.
+    #             changes (as its version counter tells: writes through
+    #             .data do not count). Routing stays as it is. bf16 and fp16
+    #             modules.
     expert_precision = "model"
 
     def _packed_weights(self, device: torch.device, dtype: torch.dtype):
@@ -308,21 +312,36 @@ class _B200Forward:
     # ---- 8-bit experts ----
     def _fp8_weights(self, device: torch.device, dtype: torch.dtype):
         """((w1, b1, w2, b2), shared [(w1, b1, w2, b2), ...]): the experts as
-        FP8Tensors with fp32 biases, made again whenever a parameter changes."""
-        w1, b1, w2, b2, sh = self._packed_weights(device, dtype)
-        key = (device, dtype) + tuple((p.data_ptr(), p._version) for p in self._expert_params())
+        FP8Tensors with fp32 biases, quantised again, into the same memory,
+        whenever a parameter's version counter or address changes (in every
+        call for parameters made in inference mode, which have no counter)."""
+        packed = self._packed_weights(device, dtype)
+        params = self._expert_params()
+        counted = not any(p.is_inference() for p in params)
+        key = (device, dtype) + tuple((p.data_ptr(), p._version if counted else None) for p in params)
         cache = getattr(self, "_b200_fp8", None)
-        if cache is not None and cache[0] == key:
+        if counted and cache is not None and cache[0] == key:
             return cache[1]
-        with torch.no_grad():
-            def quantise(v1, c1, v2, c2):
-                return ops.quantize_fp8_weight(v1), c1.float(), ops.quantize_fp8_weight(v2), c2.float()
-
-            shared = []
-            if sh is not None:
-                shared = [quantise(*(t[s:s + 1].contiguous() for t in sh)) for s in range(sh[0].shape[0])]
-            pack = (quantise(w1, b1, w2, b2), shared)
-        self._b200_fp8 = (key, pack)
+        if torch.cuda.is_current_stream_capturing():
+            raise MoEKernelError("the 8-bit experts are not up to date: run the module once before capturing it")
+        w1, b1, w2, b2, sh = packed
+        groups = [(w1, b1, w2, b2)]
+        if sh is not None:
+            groups += [tuple(t[s:s + 1].contiguous() for t in sh) for s in range(sh[0].shape[0])]
+        with torch.inference_mode(False), torch.no_grad():  # the biases are written again later
+            made = cache[1] if cache is not None else None
+            made = [made[0], *made[1]] if made is not None else []
+            shapes = [[t.shape for t in g] for g in groups]
+            if [[g[0].q.shape, g[1].shape, g[2].q.shape, g[3].shape] for g in made] != shapes or \
+                    (made and made[0][1].device != device):
+                made = [(None, torch.empty(g[1].shape, dtype=torch.float32, device=device),
+                         None, torch.empty(g[3].shape, dtype=torch.float32, device=device)) for g in groups]
+            pack = []
+            for (v1, c1, v2, c2), (q1, f1, q2, f2) in zip(groups, made):
+                pack.append((ops.quantize_fp8_weight(v1, out=q1), f1.copy_(c1),
+                             ops.quantize_fp8_weight(v2, out=q2), f2.copy_(c2)))
+        pack = (pack[0], pack[1:])
+        self._b200_fp8 = (key, pack, packed)  # holds the memory whose address the key names
         return pack
 
     def _forward_fp8(self, flat: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.Tensor:

@@ -630,8 +630,8 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     n, E = logits.shape
     if bias is not None:
         _need("bias", bias, torch.float32, (E,), dev)
-    idx = torch.empty(n, top_k, dtype=torch.int32, device=dev)
-    weights = torch.empty(n, top_k, dtype=torch.float32, device=dev)
+    idx = torch.empty(n, max(top_k, 0), dtype=torch.int32, device=dev)
+    weights = torch.empty(n, max(top_k, 0), dtype=torch.float32, device=dev)
     _call(dev, "agm_route_experts", logits.data_ptr(), dtype_code(logits.dtype), n, E, top_k, _score_code(score),
           _address(bias), n_groups, n_groups if top_groups is None else top_groups,
           renormalize, scale, idx.data_ptr(), weights.data_ptr())
@@ -701,16 +701,20 @@ def quantize_fp8(x: torch.Tensor) -> FP8Tensor:
     return t
 
 
-def quantize_fp8_weight(w: torch.Tensor) -> FP8Tensor:
+def quantize_fp8_weight(w: torch.Tensor, *, out: Optional[FP8Tensor] = None) -> FP8Tensor:
     """Weights [G, n, width] (nn.Linear layout) -> e4m3 with one scale per
-    128 x 128 block, chosen as in :func:`quantize_fp8`."""
+    128 x 128 block, chosen as in :func:`quantize_fp8`; into ``out`` when given."""
     dev = _cuda_matrix("w", w, 3)
     G, n, width = w.shape
-    t = FP8Tensor(torch.empty(G, n, width, dtype=torch.float8_e4m3fn, device=dev),
-                  torch.empty(G, *_scale_shape(n, width), dtype=torch.uint8, device=dev))
-    _call(dev, "agm_quantize_fp8_weight", w.data_ptr(), dtype_code(w.dtype), G, n, width, t.q.data_ptr(),
-          t.scales.data_ptr())
-    return t
+    if out is None:
+        out = FP8Tensor(torch.empty(G, n, width, dtype=torch.float8_e4m3fn, device=dev),
+                        torch.empty(G, *_scale_shape(n, width), dtype=torch.uint8, device=dev))
+    else:
+        _need_fp8("out", out, 3, dev)
+        _need("out.q", out.q, torch.float8_e4m3fn, (G, n, width), dev)
+    _call(dev, "agm_quantize_fp8_weight", w.data_ptr(), dtype_code(w.dtype), G, n, width, out.q.data_ptr(),
+          out.scales.data_ptr())
+    return out
 
 
 def dequantize_fp8(t: FP8Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:

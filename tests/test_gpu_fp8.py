@@ -405,6 +405,55 @@ def test_module_with_8_bit_experts(top_k, shared, residual):
         m(x)
 
 
+def test_module_8_bit_copies_follow_the_parameters():
+    """Captured, replayed after a change, first run in inference mode, with replaced parameters."""
+    torch.manual_seed(5)
+    d, E, n, dtype = 256, 4, 40, torch.bfloat16
+    x = acts(n, d, 4, dtype)
+
+    def module():
+        m = agillm41_b200.MoEFFN(d, mlp_mult=2, experts=E, top_k=2, shared_experts=1, shared_mlp_mult=1)
+        m = m.to(device="cuda", dtype=dtype).eval()
+        m.expert_precision = "fp8"
+        return m
+
+    def fresh(m):
+        c = module()
+        c.load_state_dict(m.state_dict())
+        return c(x)
+
+    m = module()
+    with torch.no_grad():
+        with pytest.raises(agillm41_b200.MoEKernelError):      # nothing to capture yet
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                m(x)
+        first = m(x)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = m(x)
+        g.replay()
+        assert torch.equal(out, first)
+        m.experts[1][0].weight.mul_(1.5)
+        m.shared[0][2].bias.add_(0.5)
+        got = m(x)
+        assert not torch.equal(got, first) and torch.equal(got, fresh(m))
+        g.replay()                                             # reads the same memory
+        assert torch.equal(out, got)
+        for _ in range(3):                                     # new parameters, perhaps at an old one's address
+            m.experts[2][2].weight = torch.nn.Parameter(torch.randn(d, 2 * d, device="cuda").to(dtype) * 0.05)
+            assert torch.equal(m(x), fresh(m))
+    m = module()
+    with torch.inference_mode():
+        first = m(x).clone()
+    with torch.no_grad():
+        assert torch.equal(m(x), first)
+        m.experts[0][0].bias.add_(0.5)
+        assert torch.equal(m(x), fresh(m)) and not torch.equal(m(x), first)
+        m.router.weight.mul_(0.5)
+    with torch.inference_mode():
+        assert torch.equal(m(x), fresh(m))
+
+
 def test_torch_operators_match():
     n, E, k, d, H = 70, 9, 3, 144, 272
     x = acts(n, d, 1, torch.float16)
@@ -418,6 +467,17 @@ def test_torch_operators_match():
     one = ops.FP8Tensor(w1.q[:1].contiguous(), w1.scales[:1].contiguous())
     assert torch.equal(o.grouped_gemm_fp8(*q, *one, b1[:1], True, None, None, torch.float16),
                        ops.grouped_gemm_fp8(ops.FP8Tensor(*q), one, b1[:1], relu=True, out_dtype=torch.float16))
+
+
+def test_quantize_weight_into():
+    w = weight(3, 80, 272, 1).bfloat16()
+    out = ops.quantize_fp8_weight(weight(3, 80, 272, 2))
+    again = ops.quantize_fp8_weight(w, out=out)
+    ref = ops.quantize_fp8_weight(w)
+    assert again.q.data_ptr() == out.q.data_ptr()
+    assert torch.equal(again.q.view(torch.uint8), ref.q.view(torch.uint8)) and torch.equal(again.scales, ref.scales)
+    with pytest.raises(agillm41_b200.MoEKernelError):
+        ops.quantize_fp8_weight(w[:2], out=out)
 
 
 def test_refusals_on_the_gpu():

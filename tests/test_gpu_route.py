@@ -253,6 +253,15 @@ def test_autograd(dtype):
         assert not route_experts(x, 4)[1].requires_grad
 
 
+def test_autograd_once():
+    """A second derivative is refused, not taken as zero."""
+    x = make(5, 9).requires_grad_()
+    _, w = route_experts(x, 2)
+    g, = torch.autograd.grad(w.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 def test_routing_then_experts():
     """A run of the operators together: router logits, grouped sigmoid routing with a balance bias, 8-bit experts,
     and the gradient back to the router."""
