@@ -206,7 +206,9 @@ class _RouteNode(torch.autograd.Function):
 def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Optional[torch.Tensor] = None,
                   n_groups: int = 1, top_groups: Optional[int] = None, renormalize: bool = True, scale: float = 1.0):
     """:func:`ops.route_experts` with autograd: router logits [N, E] ->
-    (idx int32 [N, k], weights fp32 [N, k]), differentiable in the logits."""
+    (idx int32 [N, k], weights fp32 [N, k]), differentiable (once) in the
+    logits. As for every autograd node, a backward pass is captured into a CUDA
+    graph only while no eager graph of the same leaves is alive."""
     return _RouteNode.apply(logits.contiguous(), None if bias is None else bias.detach(), top_k, score, n_groups,
                             top_groups, renormalize, scale)
 
