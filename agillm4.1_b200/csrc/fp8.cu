@@ -134,25 +134,27 @@ struct UnitWalk {
 };
 
 // Units of a warp in flight: one at a time, 94 M elements of bf16 took 78 us to
-// quantise and 65 us to read back; four at a time 56 and 54 us.
+// quantise and 65 us to read back; four at a time 56 and 54 us. fp32 takes the
+// registers of two of them for one (90 us on four, 82 on three, 77 on two).
 constexpr int kFlight = 4;
 
 // One warp per (row, 512 columns); rows up to the next multiple of 128 get a
 // scale word only, so that whole scale tiles are defined. Bound by memory:
 // 73,728 x 1280 bf16 in 52 us, 283 MB at 5.4 TB/s, with 61% of the issue slots
-// taken.
+// taken; fp32 in 77 us, 472 MB at 6.1 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 3)
     quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int width, int width_k4, uint8_t* __restrict__ q,
                          uint8_t* __restrict__ scales) {
+  constexpr int FLIGHT = sizeof(T) == 4 ? kFlight / 2 : kFlight;
   const int lane = lane_id();
   const int64_t all_rows = (rows + 127) / 128 * 128;
   UnitWalk w(static_cast<int64_t>(blockIdx.x) * kWarps + warp_id(), static_cast<int64_t>(gridDim.x) * kWarps, width_k4);
   while (w.row < all_rows) {
-    Raw16<T> raw[kFlight];
+    Raw16<T> raw[FLIGHT];
     UnitWalk ahead = w;
 #pragma unroll
-    for (int i = 0; i < kFlight; ++i) {
+    for (int i = 0; i < FLIGHT; ++i) {
       const int c = ahead.k4 * 512 + lane * 16;
       if (ahead.row < rows && c < width)
         raw[i].load(x + ahead.row * width + c);
@@ -161,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 3)
       ahead.next();
     }
 #pragma unroll
-    for (int i = 0; i < kFlight; ++i) {
+    for (int i = 0; i < FLIGHT; ++i) {
       if (w.row < all_rows) {
         float v[16];
         raw[i].unpack(v);
