@@ -565,19 +565,29 @@ __global__ void __launch_bounds__(kThreads)
                             const float* __restrict__ weights, int64_t n, int nchunk, int k,
                             const T* __restrict__ residual, T* __restrict__ out) {
   static_assert(ONE || P == 1, "several parts only for few rows");
-  pdl_wait();
-  pdl_trigger();
   const int lane = lane_id();
   const uint4* y4 = reinterpret_cast<const uint4*>(y);
   const uint4* res4 = reinterpret_cast<const uint4*>(residual);
   const int parts = (nchunk + 32 * P - 1) / (32 * P);
   const int64_t units = n * parts;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + warp_id(); u < units; u += step) {
+  int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + warp_id();
+  int my_row = -1;
+  float my_w = 0.f;
+  auto fetch = [&]() {
+    if (u >= units || lane >= k) return;
+    const int64_t t = parts == 1 ? u : u / parts;
+    my_row = row_of[t * k + lane];
+    my_w = weights[t * k + lane];
+  };
+  // Rows and weights come from before the launch that this one overlaps with
+  // (the product that writes y), which had waited for them.
+  fetch();
+  pdl_wait();
+  pdl_trigger();
+  for (; u < units; u += step, fetch()) {
     const int64_t t = parts == 1 ? u : u / parts;
     const int c0 = static_cast<int>(u - t * parts) * 32 * P + lane;
-    const int my_row = lane < k ? row_of[t * k + lane] : -1;
-    const float my_w = lane < k ? weights[t * k + lane] : 0.f;
     float acc[8];
     auto start = [&](int c) {
 #pragma unroll

@@ -633,6 +633,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   pdl_wait();
   pdl_trigger();
+  int first_ticket = blockIdx.x;
+  if (FUSED && threadIdx.x == 0) first_ticket = atomicAdd(args.ticket, 1);  // answered while the groups are read
   load_groups(args.p[0], kWRows, grp);
   tc_fence_before();
   __syncthreads();
@@ -675,13 +677,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- TMA producer ----------------
     int stage = 0;
     uint32_t phase = 0, armed = 0, armed_parity = 0;
-    int drawn = 0, ahead = 0;
-    if (FUSED) {
-      if (lane == 0) ahead = atomicAdd(args.ticket, 1);
-      ahead = __shfl_sync(0xffffffffu, ahead, 0);
-    } else {
-      ahead = blockIdx.x;
-    }
+    int drawn = 0, ahead = __shfl_sync(0xffffffffu, first_ticket, 0);
     bool ok = true;
     while (ok) {
       const int t = ahead < total ? ahead : -1;
