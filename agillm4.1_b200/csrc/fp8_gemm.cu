@@ -854,8 +854,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int acc = it & 1;
       const int n0 = u.nb * 128;
       const int live = min(u.valid, kWRows);
-      // Rows this unit writes: its live rows, and behind a segment's last row zeros up to the next multiple of 128.
-      const int rows = (g.zero_pad && u.valid <= kWRows) ? live + ((-(u.row0 + live)) & 127) : live;
+      // Rows this unit writes: its live rows, and behind a segment's last row zeros up to the next multiple of 128
+      // or the last row there is.
+      const int rows = (g.zero_pad && u.valid <= kWRows)
+                           ? static_cast<int>(min(static_cast<int64_t>(live + ((-(u.row0 + live)) & 127)), g.a_rows - u.row0))
+                           : live;
       const int chunks = (live + 31) / 32;
       const int out_k4 = scale_k4(g.n);
       const bool in_n = n0 + quarter * 32 + lane < g.n;

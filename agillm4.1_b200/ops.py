@@ -740,7 +740,7 @@ def grouped_gemm_fp8(a: FP8Tensor, w: FP8Tensor, bias: Optional[torch.Tensor] = 
     of 16, G <= 512. ``seg_start`` int32 [G + 1] and ``counts`` int32 [G]: group
     g holds the rows [seg_start[g], seg_start[g] + counts[g]); segments start
     at multiples of 128 and do not overlap. The rows behind a group's last, up
-    to the next multiple of 128, come back as zeros; other rows of the output
+    to the next multiple of 128 or R, come back as zeros; other rows of the output
     are not written (``out`` keeps them). Without them G is 1 and every row
     belongs to the group.
 

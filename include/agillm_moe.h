@@ -554,7 +554,7 @@ AGM_API int agm_dequantize_fp8(const void* q, const void* scales, int64_t groups
  *   seg_start int32 [groups + 1], counts int32 [groups] (device): group g's
  *     rows are [seg_start[g], seg_start[g] + counts[g]); seg_start are
  *     multiples of 128 and segments do not overlap. A segment's rows behind
- *     its count, up to the next multiple of 128, are written as zeros; all
+ *     its count, up to the next multiple of 128 or the last row, are zeros; all
  *     other rows of c are left as they were. Both null: groups is 1 and the
  *     group holds all a_rows rows.
  *   c [a_rows, n_out]: c_dtype AGM_BF16 or AGM_F16; or, with c_scales, e4m3

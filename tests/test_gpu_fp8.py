@@ -198,6 +198,27 @@ def test_product_keeps_nan(mode):
     assert bool(torch.isnan(y[7]).all()) and int(torch.isnan(y).any(1).sum()) == 1
 
 
+@pytest.mark.parametrize("mode", [WEIGHTS, ROWS])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_product_rows_that_end_inside_a_tile(out_dtype, mode):
+    """The last segment's 128 rows need not all exist: nothing is written behind the last row."""
+    counts, R, N, K = [130, 3, 70], 640 - 57, 144, 256
+    seg, cnt, start = segments(counts)
+    a, w = ops.quantize_fp8(acts(R, K, 1)), ops.quantize_fp8_weight(weight(3, N, K, 2))
+    assert start[2] + counts[2] < R < start[3] + 128
+    seg[2], cnt[2] = 512, R - 512                              # the last segment holds the last row
+    for last in (R - 512, 3):
+        cnt[2] = last
+        big = torch.full((R + 200, N), 5, dtype=torch.uint8, device="cuda")
+        if out_dtype == torch.bfloat16:
+            big = big.to(out_dtype)
+        out = big.view(out_dtype)[:R]
+        y = ops.grouped_gemm_fp8(a, w, seg_start=seg, counts=cnt, out_dtype=out_dtype, mode=mode, out=out)
+        got = (fo.read(y) if out_dtype == torch.float8_e4m3fn else y).double()
+        assert bool((big[R:] == 5).all())
+        assert bool((got[512 + last:] == 0).all()) and bool((got[512:512 + last] != 0).any(1).all())
+
+
 def test_product_bad_segments_are_left_out():
     """Segments that leave the rows, or do not start at a tile, are refused on the device: the others are computed."""
     a, w = ops.quantize_fp8(acts(384, 128, 1)), ops.quantize_fp8_weight(weight(3, 128, 128, 2))
