@@ -36,7 +36,7 @@ AR/SAT/NAT inference paths and the pipeline-stage runtime construct it, and
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 import torch.nn as nn
@@ -213,6 +213,26 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
                             top_groups, renormalize, scale)
 
 
+class _Fp8Copies(NamedTuple):
+    """A module's 8-bit experts: what they were made from and where. They stay
+    behind when the module is copied or pickled."""
+    key: tuple
+    pack: tuple
+    packed: tuple  # the memory whose addresses the key names
+    stream: torch.cuda.Stream
+    made: torch.cuda.Event
+
+    def __deepcopy__(self, memo):
+        return None
+
+    def __reduce__(self):
+        return _nothing, ()
+
+
+def _nothing():
+    return None
+
+
 class _B200Forward:
     """Forward of the MoE block on the B200 kernels (mixed into the module classes)."""
 
@@ -322,8 +342,11 @@ class _B200Forward:
         counted = not any(p.is_inference() for p in params)
         key = (device, dtype) + tuple((p.data_ptr(), p._version if counted else None) for p in params)
         cache = getattr(self, "_b200_fp8", None)
-        if counted and cache is not None and cache[0] == key:
-            return cache[1]
+        stream = torch.cuda.current_stream(device)
+        if counted and cache is not None and cache.key == key:
+            if stream != cache.stream and not torch.cuda.is_current_stream_capturing():
+                stream.wait_event(cache.made)
+            return cache.pack
         if torch.cuda.is_current_stream_capturing():
             raise MoEKernelError("the 8-bit experts are not up to date: run the module once before capturing it")
         w1, b1, w2, b2, sh = packed
@@ -331,8 +354,7 @@ class _B200Forward:
         if sh is not None:
             groups += [tuple(t[s:s + 1].contiguous() for t in sh) for s in range(sh[0].shape[0])]
         with torch.inference_mode(False), torch.no_grad():  # the biases are written again later
-            made = cache[1] if cache is not None else None
-            made = [made[0], *made[1]] if made is not None else []
+            made = [] if cache is None else [cache.pack[0], *cache.pack[1]]
             shapes = [[t.shape for t in g] for g in groups]
             if [[g[0].q.shape, g[1].shape, g[2].q.shape, g[3].shape] for g in made] != shapes or \
                     (made and made[0][1].device != device):
@@ -343,7 +365,7 @@ class _B200Forward:
                 pack.append((ops.quantize_fp8_weight(v1, out=q1), f1.copy_(c1),
                              ops.quantize_fp8_weight(v2, out=q2), f2.copy_(c2)))
         pack = (pack[0], pack[1:])
-        self._b200_fp8 = (key, pack, packed)  # holds the memory whose address the key names
+        self._b200_fp8 = _Fp8Copies(key, pack, packed, stream, stream.record_event())
         return pack
 
     def _forward_fp8(self, flat: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.Tensor:

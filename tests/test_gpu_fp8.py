@@ -1,6 +1,9 @@
 """Block-scaled e4m3 on the GPU against its definition in 64 bits: quantisation
 and its inverse bit for bit, the grouped products and the experts' forward to
 bounds counted from their roundings."""
+import copy
+import io
+
 import pytest
 import torch
 
@@ -473,6 +476,36 @@ def test_module_8_bit_copies_follow_the_parameters():
         m.router.weight.mul_(0.5)
     with torch.inference_mode():
         assert torch.equal(m(x), fresh(m))
+
+
+def test_module_8_bit_copies_on_two_streams():
+    """First used on a busy stream, then at once on another; no tokens at all; copied and pickled."""
+    torch.manual_seed(6)
+    d, E, n, dtype = 1024, 8, 64, torch.bfloat16
+    m = agillm41_b200.MoEFFN(d, mlp_mult=2, experts=E, top_k=2).to(device="cuda", dtype=dtype).eval()
+    m.expert_precision = "fp8"
+    x = acts(n, d, 4, dtype)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    busy = torch.randn(4096, 4096, device="cuda")
+    with torch.no_grad():
+        m._packed_weights(x.device, dtype)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(a):
+            for _ in range(20):
+                busy = busy @ busy * 1e-4
+            first = m(x)
+        with torch.cuda.stream(b):
+            second = m(x)
+        torch.cuda.synchronize()
+        assert torch.equal(first, m(x)) and torch.equal(second, first)
+        assert m(x[:0]).shape == (0, d)
+        twin = copy.deepcopy(m)
+        twin.experts[0][0].weight.mul_(2)
+        assert not torch.equal(twin(x), first) and torch.equal(m(x), first)
+        blob = io.BytesIO()
+        torch.save(m, blob)
+        blob.seek(0)
+        assert torch.equal(torch.load(blob, weights_only=False)(x), first)
 
 
 def test_torch_operators_match():
