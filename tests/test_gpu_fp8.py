@@ -236,6 +236,30 @@ def test_product_bad_segments_are_left_out():
             assert bool((out[128:256] == 3).all()) and bool((out[:10] != 3).any()) and bool((out[256:266] != 3).any())
 
 
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the end comes out as it does on its own."""
+    R, W, N = 1_700_001, 1296, 1312
+    x = torch.empty(R, W, dtype=torch.bfloat16, device="cuda").normal_(generator=gen(1))
+    s = R // 128 * 128 - 1280
+    q, p = ops.quantize_fp8(x), ops.quantize_fp8(x[s:].contiguous())
+    assert torch.equal(q.q[s:].view(torch.uint8), p.q.view(torch.uint8)) and torch.equal(q.scales[s // 128:], p.scales)
+    assert torch.equal(ops.dequantize_fp8(q)[s:], ops.dequantize_fp8(p))
+    w = ops.quantize_fp8_weight(weight(1, N, W, 2))
+    for mode in (ROWS, WEIGHTS):
+        assert torch.equal(ops.grouped_gemm_fp8(q, w, mode=mode)[s:], ops.grouped_gemm_fp8(p, w, mode=mode))
+        y, z = (ops.grouped_gemm_fp8(t, w, mode=mode, out_dtype=torch.float8_e4m3fn) for t in (q, p))
+        assert torch.equal(y.q[s:].view(torch.uint8), z.q.view(torch.uint8)) and torch.equal(y.scales[s // 128:], z.scales)
+        del y, z
+    del q, p
+    n, E, d, H = 1_100_000, 16, 1024, 256
+    x = x.view(-1)[:n * d].view(n, d)
+    idx, wgt = ops.route_experts(torch.randn(n, E, generator=gen(3), device="cuda"), 2)
+    wts = make_experts(E, d, H, 4)
+    out = ops.moe_experts_fp8(x, idx, wgt, *wts, check_errors=True)
+    tail = (t[-4000:].contiguous() for t in (x, idx, wgt))
+    assert torch.equal(out[-4000:], ops.moe_experts_fp8(*tail, *wts))
+
+
 # ---------------------------------------------------------------------------
 # The experts' forward
 # ---------------------------------------------------------------------------

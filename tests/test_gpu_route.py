@@ -109,6 +109,19 @@ def test_many_tokens():
         check(x, 6, score="softmax", n_groups=16, top_groups=3, renormalize=False)
 
 
+@pytest.mark.parametrize("kw", [dict(top_k=8, score="sigmoid", n_groups=8, top_groups=4), dict(top_k=12), dict(top_k=6)])
+def test_offsets_past_32_bits(kw):
+    """More than 2^31 logits: the last rows come out as they do on their own."""
+    x = torch.empty(9_000_003, 256, dtype=torch.bfloat16, device="cuda").normal_(generator=gen(5))
+    last = x[-5000:].contiguous()
+    score = kw.get("score", "softmax")
+    idx, w = ops.route_experts(x, **kw)
+    idx2, w2 = ops.route_experts(last, **kw)
+    assert torch.equal(idx[-5000:], idx2) and torch.equal(w[-5000:], w2)
+    d = ops.route_experts_backward(w, x, idx, score=score)
+    assert torch.equal(d[-5000:], ops.route_experts_backward(w2, last, idx2, score=score))
+
+
 def test_ties_go_to_the_lowest_index():
     x = torch.zeros(5, 48, device="cuda")
     x[1, 7] = x[1, 30] = x[1, 44] = 2.0
