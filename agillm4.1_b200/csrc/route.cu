@@ -499,13 +499,24 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
           for (int j = 0; j < SB; ++j) s[j] += bias_s[sub * LD + b * SB + j];
         }
       }
+      float h[SB], w[SB];  // the two largest of 2, 4, ... keys
 #pragma unroll
       for (int j = 0; j < SB; ++j) {
         const float c = key[b * SB + j] == kNegInf ? kNegInf : s[j];
-        k2 = fmaxf(k2, fminf(k1, c));
-        k1 = max_nan(k1, c);
         key[b * SB + j] = c;
+        h[j] = c;
+        w[j] = kNegInf;
       }
+#pragma unroll
+      for (int o = 1; o < SB; o <<= 1)
+#pragma unroll
+        for (int j = 0; j + o < SB; j += 2 * o) {
+          const float mid = fminf(h[j], h[j + o]);
+          w[j] = o == 1 ? mid : fmaxf(fmaxf(w[j], w[j + o]), mid);
+          h[j] = max_nan(h[j], h[j + o]);
+        }
+      k1 = h[0];
+      k2 = w[0];
     } else {
 #pragma unroll
       for (int j = 0; j < SB; ++j) k1 = max_nan(k1, key[b * SB + j]);
@@ -628,17 +639,29 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
   for (int at = upto - count; hit && at < kWideList; ++at) {
     const int j = __ffs(hit) - 1;
     hit &= hit - 1;
-    float v = my_logit[j];
-    if (biased) {
-      v = sigmoid ? fast_rcp(1.f + fast_exp(-v)) : fast_exp(v - m) * inv_t;  // as in 2
-      v += bias_s[sub * LD + j];
-    }
     sm.id[tok][at] = sub * per + j;
-    sm.key[tok][at] = v + 0.f;  // -0 = 0
+    sm.key[tok][at] = RAW ? my_logit[j] + 0.f : __int_as_float(sub * LD + j);  // -0 = 0; or its place
   }
   const int len = min(total, kWideList);
   const int len4 = (len + 3) & ~3;
-  for (int i = len + sub; i < len4; i += L) sm.key[tok][i] = kNegInf;
+  if constexpr (RAW) {
+    for (int i = len + sub; i < len4; i += L) sm.key[tok][i] = kNegInf;
+  } else {
+    // The keys again, shared out over the lanes: few hold most of the list.
+    __syncwarp();
+    for (int i = sub; i < len4; i += L) {
+      float v = kNegInf;
+      if (i < len) {
+        const int at = __float_as_int(sm.key[tok][i]);
+        v = sm.logit[tok][at];
+        if (biased) {
+          v = sigmoid ? fast_rcp(1.f + fast_exp(-v)) : fast_exp(v - m) * inv_t;  // as in 2
+          v += bias_s[at];
+        }
+      }
+      sm.key[tok][i] = v + 0.f;  // -0 = 0
+    }
+  }
   for (int i = sub; i <= kWideTopK; i += L) sm.sel[tok][i] = -1;
   __syncwarp();
   // 5. Each finds its rank: the number of keys above it.
