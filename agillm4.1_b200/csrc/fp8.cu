@@ -558,7 +558,10 @@ __global__ void __launch_bounds__(kThreads, 3) dispatch_rows_kernel(Fp8Dispatch 
 // One warp per token and P x 256 columns: a lane sums P x 8 columns over the
 // token's rows, the loads of KU rows in flight at a time. ONE: k <= KU, so
 // that only one part's sums are held at a time. Bound by memory: 73,728 tokens
-// x 1280 bf16, top-2, 567 MB in about 115 us, 4.9 TB/s.
+// x 1280 bf16, top-2, 567 MB in about 115 us, 4.9 TB/s. y comes rounded to T, as
+// the block in its own precision rounds it: fp32 would be 377 MB more to write
+// and 377 MB more to read here, some 115 us of 1.3 ms, for a relative error of
+// 0.0017 (the last rounding's) in place of 0.0023.
 template <typename T, int KU, int P, bool ONE>
 __global__ void __launch_bounds__(kThreads)
     combine_weighted_kernel(const T* __restrict__ y, const int32_t* __restrict__ row_of,
