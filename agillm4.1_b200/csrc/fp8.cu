@@ -575,20 +575,23 @@ __global__ void __launch_bounds__(kThreads)
   const int64_t units = n * parts;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
   int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + warp_id();
-  int my_row = -1;
-  float my_w = 0.f;
+  int my_row;
+  float my_w;
   auto fetch = [&]() {
-    if (u >= units || lane >= k) return;
-    const int64_t t = parts == 1 ? u : u / parts;
-    my_row = row_of[t * k + lane];
-    my_w = weights[t * k + lane];
+    const bool in = u < units && lane < k;
+    const int64_t at = (parts == 1 ? u : u / parts) * k + lane;
+    my_row = in ? row_of[at] : -1;
+    my_w = in ? weights[at] : 0.f;
   };
   // Rows and weights come from before the launch that this one overlaps with
-  // (the product that writes y), which had waited for them.
-  fetch();
+  // (the product that writes y), which had waited for them: few tokens fetch
+  // them before their own wait (0.6 us of 36 at 64 tokens); the wide form has
+  // no registers for it (a CTA fewer per SM).
+  if (P == 1) fetch();
   pdl_wait();
   pdl_trigger();
-  for (; u < units; u += step, fetch()) {
+  for (; u < units; u += step) {
+    if (P > 1 || u >= step) fetch();
     const int64_t t = parts == 1 ? u : u / parts;
     const int c0 = static_cast<int>(u - t * parts) * 32 * P + lane;
     float acc[8];
