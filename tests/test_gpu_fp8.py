@@ -404,6 +404,28 @@ def test_small_batches_at_once(n):
     assert all(torch.equal(a, b) for a, b in zip(gouts, ref))
 
 
+@pytest.mark.parametrize("n", [1, 64, 900])
+def test_one_workspace_for_calls_in_a_row(n):
+    """Launches overlap at their ends: another routing in the same workspace must not show through."""
+    E, k, d, H = 14, 2, 256, 384
+    wts = make_experts(E, d, H, 1)
+    x = acts(n, d, 2, torch.bfloat16)
+    route = [ops.route_experts(torch.randn(n, E, generator=gen(9 + i), device="cuda"), k) for i in range(3)]
+    ref = [ops.moe_experts_fp8(x, *r, *wts, check_errors=True) for r in route]
+    nbytes = _lib.load().agm_moe_experts_fp8_workspace_bytes(n, d, E, k, H)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    outs = [ops.moe_experts_fp8(x, *route[i % 3], *wts, workspace=ws) for i in range(60)]
+    assert all(torch.equal(o, ref[i % 3]) for i, o in enumerate(outs))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = [ops.moe_experts_fp8(x, *route[i % 3], *wts, workspace=ws) for i in range(12)]
+    for _ in range(5):
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, ref[i % 3]) for i, o in enumerate(outs))
+
+
 @pytest.mark.parametrize("top_k,shared,residual", [(1, 0, False), (2, 0, True), (2, 2, True), (3, 1, False)])
 def test_module_with_8_bit_experts(top_k, shared, residual):
     """MoEFFN with expert_precision "fp8" against the same routing through the definition; a changed parameter is seen."""
