@@ -463,8 +463,6 @@ __global__ void __launch_bounds__(kThreads, 3) dispatch_rows_kernel(Fp8Dispatch 
   const int lane = lane_id(), warp = warp_id();
   const int E = a.n_experts;
   const int blk = blockIdx.x / split, part = blockIdx.x - blk * split;
-  pdl_wait();
-  pdl_trigger();
   const int64_t tok0 = static_cast<int64_t>(blk) * kTokBlk;
   const int toks = static_cast<int>(min(static_cast<int64_t>(kTokBlk), a.n - tok0));
   const int slots = toks * a.k;
@@ -478,14 +476,18 @@ __global__ void __launch_bounds__(kThreads, 3) dispatch_rows_kernel(Fp8Dispatch 
   };
   const int first = part * kWarps + warp;
   Raw16<T> raw[4];
+  // The batch was there before the two launches ahead, and the second of them
+  // waited for the first: only the counts have to be waited for.
   if (first < toks) load_four(first, 0, raw);  // in flight during the ranking
-  if (warp == 0) padded_prefix(a.counts, E, start_s, lane);
   for (int e = lane; e < E; e += 32) base_s[warp][e] = 0;
   __syncwarp();
   for (int s = s0 + lane; s < s1; s += 32) {
     const int e = idx[s];
     if (e >= 0 && e < E) atomicAdd(&base_s[warp][e], 1);
   }
+  pdl_wait();
+  pdl_trigger();
+  if (warp == 0) padded_prefix(a.counts, E, start_s, lane);
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += kThreads) {
     int at = start_s[e] + a.block_hist[static_cast<int64_t>(blk) * E + e];
