@@ -233,15 +233,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tmSA);
     tma_prefetch_desc(&tmSB);
   }
-  pdl_wait();
-  pdl_trigger();
-  load_groups(args, 256, grp);
   __syncthreads();
   cluster_sync();  // both CTAs' barriers exist before any cross-CTA arrive or copy
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, 512);
     tmem_relinquish_pair();
   }
+  pdl_wait();
+  pdl_trigger();
+  load_groups(args, 256, grp);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
