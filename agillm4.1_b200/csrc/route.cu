@@ -8,8 +8,9 @@
 //   w_r = scale * s[idx_r]  (/ sum_j s[idx_j] when renormalised)
 //
 // An expert whose key is -inf or NaN is never chosen: its slot gets index -1
-// and weight 0. A NaN logit (or +inf under softmax) makes the row's weights
-// NaN.
+// and weight 0. A NaN logit takes its own expert out of the scores, and +inf
+// under softmax is the limit of a large logit (the experts that have it share
+// a score of 1), so such a row still chooses; its weights are NaN.
 //
 // The order of the keys is decided in real arithmetic: without a bias a key is
 // the logit itself, exact. Otherwise the keys are computed in fp32 (error
@@ -35,8 +36,8 @@
 //   12 for k = 8) go to a list in index order, where each finds its rank by
 //   counting. Where keys are too close to be told apart, those of the list,
 //   or the two that make a group's score, are formed again in fp64. Only rows
-//   with more than 32 keys at the border go through the other kernel's code,
-//   one by one. That case now takes 41 us: 71 MB at 1.7 TB/s, still bound by
+//   with more than 32 keys at the border, or a NaN or infinite softmax, go
+//   through the other kernel's code, one by one. That case now takes 41 us: 71 MB at 1.7 TB/s, still bound by
 //   issuing (58% of the slots at 24 warps per SM). Two CTAs per SM with 128
 //   registers took 45 us, 16 lanes a token 48, 64 registers with the keys
 //   written over the logits 47. 262,144 x 64 bf16, top-6: 47 us.
@@ -123,7 +124,8 @@ __device__ __forceinline__ bool select_experts(const float (&l)[V], const RouteA
       F t = 0;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        s[j] = l[j] > kNegInf ? exp_of(static_cast<F>(l[j]) - static_cast<F>(m)) : F(0);
+        // min: +inf - +inf is NaN, for which it gives 0
+        s[j] = l[j] > kNegInf ? exp_of(min(static_cast<F>(l[j]) - static_cast<F>(m), F(0))) : F(0);
         t += s[j];
       }
       t = lanes_sum<F, L>(t);
@@ -352,6 +354,7 @@ __device__ __forceinline__ double exact_score(float l, bool sigmoid, float m, do
 
 constexpr int kWideTopK = 8;
 constexpr int kWideList = 32;
+constexpr int kWideOdd = kWideTopK + 1;
 
 template <int L, int V>
 struct WideSmem {
@@ -363,7 +366,7 @@ struct WideSmem {
   float key[kTok][kWideList];
   int id[kTok][kWideList];
   float sorted[kTok][kWideTopK + 4];   // keys by rank, the first k + 1
-  int sel[kTok][kWideTopK + 4];        // their experts
+  int sel[kTok][kWideTopK + 4];        // their experts; at kWideOdd: the token has no finite scores
 };
 
 template <typename T>
@@ -400,6 +403,7 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
   using Smem = WideSmem<L, V>;
   constexpr int TOK = Smem::kTok, LD = Smem::kLane, SB = V / 4;
   constexpr uint32_t kAll = 0xffffffffu;
+  static_assert(sizeof(Smem) % 16 == 0, "the warps' parts are read in 16-byte units");
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Smem& sm = reinterpret_cast<Smem*>(smem_raw)[warp_id()];
   float* bias_s = reinterpret_cast<float*>(smem_raw + sizeof(Smem) * (kRouteThreads / 32));  // [L * LD]
@@ -472,6 +476,9 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
 #pragma unroll
     for (int j = 0; j < V; ++j) t += fast_exp(key[j] - m);
     t = lanes_sum<float, L>(t);
+    // t is NaN beside a NaN or +inf logit: the scores below are none then, and the other kernel's code routes the
+    // token (a flag kept in a register cost spills).
+    if (!RAW) sm.sel[tok][kWideOdd] = t != t;
     inv_t = t > 0.f ? 1.f / t : 0.f;
   }
   float top[8], g1 = kNegInf, g2 = kNegInf;
@@ -754,7 +761,8 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
       nan_row |= v != v || (!sigmoid && v == INFINITY);
     }
   }
-  if (live && !crowded) {
+  const bool alone = crowded || (!RAW && !sigmoid && sm.sel[tok][kWideOdd] != 0);
+  if (live && !alone) {
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {
       const int r = sub + L * i;
@@ -764,9 +772,9 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
       }
     }
   }
-  // 7. Tokens with more keys at the border than the list holds, one by one.
+  // 7. Tokens with more keys at the border than the list holds, or without finite scores, one by one.
   // Last, so that the call keeps nothing of the above alive.
-  for (uint32_t open = __ballot_sync(kAll, crowded && live && sub == 0); open; open &= open - 1)
+  for (uint32_t open = __ballot_sync(kAll, alone && live && sub == 0); open; open &= open - 1)
     route_one<T>(logits, a, t0 + (__ffs(open) - 1) / L, idx, weights);
 }
 

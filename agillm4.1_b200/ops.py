@@ -624,7 +624,8 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     An expert with logit -inf, or whose key is -inf or NaN, is never chosen;
     a slot left without an expert gets idx -1 and weight 0 (a token routed
     nowhere is a row of -inf). A row with a NaN logit (+inf too, under softmax)
-    gets NaN weights. The gradient is :func:`route_experts_backward`;
+    gets NaN weights and still chooses: NaN takes out its own expert only, and
+    +inf is the limit of a large logit. The gradient is :func:`route_experts_backward`;
     :func:`agillm41_b200.route_experts` is the differentiable form."""
     dev = _cuda_matrix("logits", logits)
     n, E = logits.shape

@@ -515,7 +515,8 @@ AGM_API int agm_read_device_error(int* err, int* code, void* stream);
  *   scale       factor of the weights
  * Ties go to the lowest index. An expert whose logit is -inf or whose key is
  * -inf or NaN is never chosen; a slot without an expert gets index -1 and
- * weight 0. A row with a NaN logit (or +inf under softmax) gets NaN weights. */
+ * weight 0. A row with a NaN logit (or +inf under softmax) gets NaN weights;
+ * NaN takes out its own expert only, and +inf is the limit of a large logit. */
 #define AGM_ROUTE_SOFTMAX 0
 #define AGM_ROUTE_SIGMOID 1
 #define AGM_ROUTE_MAX_EXPERTS 512

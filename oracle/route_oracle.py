@@ -9,6 +9,7 @@ def scores(l, score):
         return torch.sigmoid(l)
     m = l.amax(dim=1, keepdim=True)
     z = torch.exp(l - torch.where(torch.isinf(m) & (m < 0), torch.zeros_like(m), m))
+    z = torch.where((l == m) & (m > 0) & torch.isinf(m), torch.ones_like(z), z)   # beside +inf: the limit
     return z / z.sum(dim=1, keepdim=True).clamp_min(1e-300)
 
 

@@ -1,0 +1,55 @@
+"""Routing where scores, biases or logits leave the ordinary range: indices against the definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from agillm41_b200 import ops
+from oracle import route_oracle as ro
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = math.inf, math.nan
+LOWEST = torch.finfo(torch.float32).min
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def make(n, E, seed=0, dtype=torch.float32):
+    return (torch.randn(n, E, generator=gen(seed), device="cuda") * 1.5).to(dtype)
+
+
+# (experts, k, groups, kept): both kernels, E on both sides of 32, k on both sides of 8, group counts that are and
+# are not powers of two
+SHAPES = [(14, 2, 1, 1), (24, 4, 3, 2), (24, 8, 4, 2), (64, 8, 1, 1), (64, 4, 8, 4), (64, 12, 8, 4), (96, 6, 3, 2),
+          (256, 8, 1, 1), (256, 8, 8, 4), (256, 12, 1, 1)]
+
+
+@pytest.mark.parametrize("E,k,groups,keep", SHAPES)
+@pytest.mark.parametrize("biased", [False, True])
+def test_nan_and_inf_logits_leave_the_others_alone(E, k, groups, keep, biased):
+    """Under softmax too, a NaN logit takes out its own expert only, +inf is the limit of a large logit, and the
+    row's weights are NaN, which the experts pass on."""
+    n = 12
+    x = make(n, E, E + k)
+    x[1, 3] = NAN
+    x[2, E - 1] = NAN
+    x[2, :E // 2:3] = NAN
+    x[3, 5] = INF
+    x[4, 1] = x[4, E - 2] = INF
+    x[5, 2], x[5, 7] = INF, NAN
+    x[6, 4], x[6, 0] = NAN, -INF
+    b = torch.randn(E, generator=gen(1), device="cuda") * 0.1 if biased else None
+    for score in ("softmax", "sigmoid"):
+        idx, w = ops.route_experts(x, k, score=score, bias=b, n_groups=groups, top_groups=keep)
+        assert torch.equal(idx.long(), ro.choose(x, k, score, b, groups, keep))
+        odd = torch.isnan(x).any(1) | ((x == INF).any(1) if score == "softmax" else False)
+        assert torch.equal(torch.isnan(w).all(1), odd) and torch.equal(torch.isnan(w).any(1), odd)
+        d, H = 64, 128
+        w1 = ops.quantize_fp8_weight(torch.randn(E, H, d, generator=gen(2), device="cuda"))
+        w2 = ops.quantize_fp8_weight(torch.randn(E, d, H, generator=gen(3), device="cuda"))
+        y = ops.moe_experts_fp8(torch.ones(n, d, device="cuda", dtype=torch.bfloat16), idx, w, w1,
+                                torch.zeros(E, H, device="cuda"), w2, torch.zeros(E, d, device="cuda"))
+        assert torch.equal(torch.isnan(y).all(1), odd) and torch.equal(torch.isnan(y).any(1), odd)
