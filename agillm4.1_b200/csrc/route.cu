@@ -565,15 +565,16 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
     const float close = (sigmoid ? 20.f : 32.f) * 0x1p-24f * (1.f + fabsf(score));
     int rank = 0;
     for (int o = span; o < L; o += span) {
-      const float so = __shfl_sync(kAll, score, (lane & ~(L - 1)) | ((sub + o) & (L - 1)));
-      rank += so > score;
+      const int other = (sub + o) & (L - 1);
+      const float so = __shfl_sync(kAll, score, (lane & ~(L - 1)) | other);
+      rank += so > score || (so == score && other < sub);  // +inf of forced experts: by index
       near |= fabsf(so - score) <= close;
     }
     if (__any_sync(kAll, near)) {
       // The group scores again, from the exact keys of the one or two (more
       // only where they are close) largest in every lane.
       need_sum();
-      const float cut = lane2 - (sigmoid ? 20.f : 64.f) * 0x1p-24f * (1.f + fabsf(lane2));
+      const float cut = lane2 == INFINITY ? lane2 : lane2 - (sigmoid ? 20.f : 64.f) * 0x1p-24f * (1.f + fabsf(lane2));
       uint32_t pair = 0;
 #pragma unroll
       for (int j = 0; j < V; ++j) mark_if_ge(pair, key[j], lane2 > kNegInf ? cut : -FLT_MAX, 1u << j);

@@ -53,3 +53,27 @@ def test_nan_and_inf_logits_leave_the_others_alone(E, k, groups, keep, biased):
         y = ops.moe_experts_fp8(torch.ones(n, d, device="cuda", dtype=torch.bfloat16), idx, w, w1,
                                 torch.zeros(E, H, device="cuda"), w2, torch.zeros(E, d, device="cuda"))
         assert torch.equal(torch.isnan(y).all(1), odd) and torch.equal(torch.isnan(y).any(1), odd)
+
+
+# (experts, groups, kept)
+GROUPS = [(32, 8, 3), (64, 8, 4), (64, 32, 3), (60, 30, 3), (48, 3, 2), (256, 8, 4), (512, 16, 4)]
+
+
+@pytest.mark.parametrize("E,groups,keep", GROUPS)
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_infinite_biases_force_experts(E, groups, keep, score):
+    """A bias of +inf puts its expert, and its group, before every finite one; equal ones go by index."""
+    x = make(40, E, E)
+    size = E // groups
+    none = torch.zeros(E, device="cuda")
+    pair, each, some, far = none.clone(), none.clone(), none.clone(), none.clone()
+    pair[:2] = INF                                   # two in one group
+    each[::size] = INF                               # one in every group
+    some[size - 1:size + 1] = some[E - 1] = INF      # three in three groups
+    far[E - size:E - size + 2] = INF
+    far[0] = -INF
+    for bias in (pair, each, some, far):
+        for k in (2, 6, 8, 9):
+            idx, w = ops.route_experts(x, k, score=score, bias=bias, n_groups=groups, top_groups=keep)
+            assert torch.equal(idx.long(), ro.choose(x, k, score, bias, groups, keep))
+            assert bool(torch.isfinite(w).all())
