@@ -100,6 +100,20 @@ __device__ __forceinline__ void lanes_best(F& v, int& id) {
   }
 }
 
+// Whether the order of real numbers may keep other groups than the fp32 scores
+// (one a lane) do. `size_of` is the sum of the magnitudes of the score's two
+// keys: each is off by its score's error, half of `error` * 2^-24, and by the
+// rounding of the bias' add, and their sum and the ends here by a rounding
+// each, which is 3 size_of 2^-24 in all (keys of opposite signs cancel in the
+// score, not in its error). Infinite scores are exact.
+template <int L>
+__device__ __forceinline__ bool groups_near(float score, float size_of, float error, bool kept) {
+  const float e = fabsf(score) < INFINITY ? (error + 4.f * size_of) * 0x1p-24f : 0.f;
+  const float hi = lanes_max<float, L>(kept ? kNegInf : score + e);
+  const float lo = -lanes_max<float, L>(kept && score > kNegInf ? e - score : kNegInf);
+  return !(lo > hi) && hi > kNegInf;
+}
+
 // Selects one token's experts; slot r = sub + L * i of lane `sub` gets sel[i].
 // Returns whether the fp32 keys leave the choice open.
 template <typename F, int L, int V, int KS>
@@ -144,7 +158,7 @@ __device__ __forceinline__ bool select_experts(const float (&l)[V], const RouteA
         int grp[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) grp[j] = (sub + L * j) / size;
-        F mine = F(kNegInf);  // lane g: score of group g
+        F mine = F(kNegInf), size_of = F(0);  // lane g: score of group g, and the magnitudes that went into it
         for (int g = 0; g < a.n_groups; ++g) {
           F t1 = F(kNegInf), t2 = F(kNegInf);
 #pragma unroll
@@ -160,22 +174,20 @@ __device__ __forceinline__ bool select_experts(const float (&l)[V], const RouteA
             t2 = max(min(t1, o1), max(t2, o2));
             t1 = max(t1, o1);
           }
-          if (sub == g) mine = t2 > F(kNegInf) ? t1 + t2 : t1;
+          if (sub == g) {
+            mine = t2 > F(kNegInf) ? t1 + t2 : t1;
+            size_of = fabs(t1) + (t2 > F(kNegInf) ? fabs(t2) : F(0));
+          }
         }
         uint32_t kept = 0;
-        F last = 0;
-        for (int i = 0; i <= a.top_groups; ++i) {
+        for (int i = 0; i < a.top_groups; ++i) {
           F v = ((kept >> sub) & 1u) ? F(kNegInf) : mine + F(0);
           int id = sub;
           lanes_best<F, 32>(v, id);
           if (!(v > F(kNegInf))) break;
-          if (i == a.top_groups) {
-            near = kFast && last - v <= F(3.8e-6f) * (F(1) + fabs(v));  // 2^-18
-            break;
-          }
           kept |= 1u << id;
-          last = v;
         }
+        if constexpr (kFast) near = groups_near<32>(mine, size_of, 32.f, (kept >> sub) & 1u);
 #pragma unroll
         for (int j = 0; j < V; ++j)
           if (!((kept >> (grp[j] & 31)) & 1u)) key[j] = F(kNegInf);
@@ -315,10 +327,9 @@ __device__ __noinline__ void route_one(const T* __restrict__ logits, const Route
 // rounded argument) and reciprocal (2^-23). A sigmoid 1 / (1 + e^-l) formed
 // from them is off by at most s (1 - s) times the exponential's error, which
 // is below 1.4 * 2^-24, plus s * 3 * 2^-24: two keys by 10 * 2^-24 (1 + |c|)
-// together with the bias' add, two sums of two by twice that. A softmax score
-// s is off by at most 30 s 2^-24 (the sum's terms and tree for E <= 512), and
-// all scores sum to 1, so two keys, or two sums of two, by
-// 32 * 2^-24 (1 + |c|).
+// together with the bias' add. A softmax score s is off by at most 30 s 2^-24
+// (the sum's terms and tree for E <= 512), and all scores sum to 1, so two
+// keys by 32 * 2^-24 (1 + |c|). For sums of two see groups_near.
 __device__ __forceinline__ float fast_exp(float v) {
   float o;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(o) : "f"(v * 1.4426950408889634f));
@@ -562,14 +573,14 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
       g1 = fmaxf(g1, o1);
     }
     const float score = g2 > kNegInf ? g1 + g2 : g1;
-    const float close = (sigmoid ? 20.f : 32.f) * 0x1p-24f * (1.f + fabsf(score));
+    const float size_of = fabsf(g1) + (g2 > kNegInf ? fabsf(g2) : 0.f);
     int rank = 0;
     for (int o = span; o < L; o += span) {
       const int other = (sub + o) & (L - 1);
       const float so = __shfl_sync(kAll, score, (lane & ~(L - 1)) | other);
-      rank += so > score || (so == score && other < sub);  // +inf of forced experts: by index
-      near |= fabsf(so - score) <= close;
+      rank += so > score || (so == score && other < sub);
     }
+    near = groups_near<L>(score, size_of, sigmoid ? 10.f : 16.f, rank < a.top_groups);
     if (__any_sync(kAll, near)) {
       // The group scores again, from the exact keys of the one or two (more
       // only where they are close) largest in every lane.

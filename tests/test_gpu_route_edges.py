@@ -77,3 +77,21 @@ def test_infinite_biases_force_experts(E, groups, keep, score):
             idx, w = ops.route_experts(x, k, score=score, bias=bias, n_groups=groups, top_groups=keep)
             assert torch.equal(idx.long(), ro.choose(x, k, score, bias, groups, keep))
             assert bool(torch.isfinite(w).all())
+
+
+@pytest.mark.parametrize("E,groups,keep,k", [(64, 32, 16, 4), (60, 30, 15, 4), (256, 8, 4, 4), (256, 8, 4, 12), (512, 32, 5, 8)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_group_scores_that_cancel(E, groups, keep, k, score):
+    """Large biases of both signs: a group's score is the small difference of large keys, whose rounding decides."""
+    x = make(20000, E, E + k)
+    size = E // groups
+    for B in (16.0, 100.0, 1000.0, 1e5, 1e30):
+        b = torch.full((E,), -B, device="cuda")
+        b[::size] = B
+        b += (torch.randn(E, generator=gen(3), device="cuda") * 0.01)
+        idx, _ = ops.route_experts(x, k, score=score, bias=b, n_groups=groups, top_groups=keep)
+        assert torch.equal(idx.long(), ro.choose(x, k, score, b, groups, keep)), B
+        b = torch.full((E,), -B, device="cuda")
+        b[::size] = B
+        idx, _ = ops.route_experts(x, k, score=score, bias=b, n_groups=groups, top_groups=keep)
+        assert torch.equal(idx.long(), ro.choose(x, k, score, b, groups, keep)), B
