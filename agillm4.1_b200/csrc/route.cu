@@ -101,8 +101,9 @@ __device__ __forceinline__ void lanes_best(F& v, int& id) {
 }
 
 // Whether the order of real numbers may keep other groups than the fp32 scores
-// (one a lane) do. `size_of` is the sum of the magnitudes of the score's two
-// keys: each is off by its score's error, half of `error` * 2^-24, and by the
+// (one a lane) do. They are half scores, h1 + h2 of the halved keys, since the
+// sum of two keys near 3.4e38 is no fp32 number; `size_of` is |h1| + |h2|. A
+// half key is off by its expert's score, `error` / 2 * 2^-24 at most, and by the
 // rounding of the bias' add, and their sum and the ends here by a rounding
 // each, which is 3 size_of 2^-24 in all (keys of opposite signs cancel in the
 // score, not in its error). Infinite scores are exact.
@@ -158,7 +159,7 @@ __device__ __forceinline__ bool select_experts(const float (&l)[V], const RouteA
         int grp[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) grp[j] = (sub + L * j) / size;
-        F mine = F(kNegInf), size_of = F(0);  // lane g: score of group g, and the magnitudes that went into it
+        F mine = F(kNegInf), size_of = F(0);  // lane g: half the score of group g, and the magnitudes that went into it
         for (int g = 0; g < a.n_groups; ++g) {
           F t1 = F(kNegInf), t2 = F(kNegInf);
 #pragma unroll
@@ -175,8 +176,9 @@ __device__ __forceinline__ bool select_experts(const float (&l)[V], const RouteA
             t1 = max(t1, o1);
           }
           if (sub == g) {
-            mine = t2 > F(kNegInf) ? t1 + t2 : t1;
-            size_of = fabs(t1) + (t2 > F(kNegInf) ? fabs(t2) : F(0));
+            const F h1 = F(0.5) * t1, h2 = F(0.5) * t2;
+            mine = t2 > F(kNegInf) ? h1 + h2 : h1;
+            size_of = fabs(h1) + (t2 > F(kNegInf) ? fabs(h2) : F(0));
           }
         }
         uint32_t kept = 0;
@@ -187,7 +189,7 @@ __device__ __forceinline__ bool select_experts(const float (&l)[V], const RouteA
           if (!(v > F(kNegInf))) break;
           kept |= 1u << id;
         }
-        if constexpr (kFast) near = groups_near<32>(mine, size_of, 32.f, (kept >> sub) & 1u);
+        if constexpr (kFast) near = groups_near<32>(mine, size_of, 16.f, (kept >> sub) & 1u);
 #pragma unroll
         for (int j = 0; j < V; ++j)
           if (!((kept >> (grp[j] & 31)) & 1u)) key[j] = F(kNegInf);
@@ -572,20 +574,21 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
       g2 = fmaxf(fminf(g1, o1), fmaxf(g2, o2));
       g1 = fmaxf(g1, o1);
     }
-    const float score = g2 > kNegInf ? g1 + g2 : g1;
-    const float size_of = fabsf(g1) + (g2 > kNegInf ? fabsf(g2) : 0.f);
+    const float h1 = 0.5f * g1, h2 = 0.5f * g2;
+    const float score = g2 > kNegInf ? h1 + h2 : h1;
+    const float size_of = fabsf(h1) + (g2 > kNegInf ? fabsf(h2) : 0.f);
     int rank = 0;
     for (int o = span; o < L; o += span) {
       const int other = (sub + o) & (L - 1);
       const float so = __shfl_sync(kAll, score, (lane & ~(L - 1)) | other);
       rank += so > score || (so == score && other < sub);
     }
-    near = groups_near<L>(score, size_of, sigmoid ? 10.f : 16.f, rank < a.top_groups);
+    near = groups_near<L>(score, size_of, sigmoid ? 5.f : 8.f, rank < a.top_groups);
     if (__any_sync(kAll, near)) {
       // The group scores again, from the exact keys of the one or two (more
       // only where they are close) largest in every lane.
       need_sum();
-      const float cut = lane2 == INFINITY ? lane2 : lane2 - (sigmoid ? 20.f : 64.f) * 0x1p-24f * (1.f + fabsf(lane2));
+      const float cut = lane2 == INFINITY ? lane2 : fmaxf(lane2 - (sigmoid ? 20.f : 64.f) * 0x1p-24f * (1.f + fabsf(lane2)), -FLT_MAX);
       uint32_t pair = 0;
 #pragma unroll
       for (int j = 0; j < V; ++j) mark_if_ge(pair, key[j], lane2 > kNegInf ? cut : -FLT_MAX, 1u << j);

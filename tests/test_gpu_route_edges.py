@@ -95,3 +95,30 @@ def test_group_scores_that_cancel(E, groups, keep, k, score):
         b[::size] = B
         idx, _ = ops.route_experts(x, k, score=score, bias=b, n_groups=groups, top_groups=keep)
         assert torch.equal(idx.long(), ro.choose(x, k, score, b, groups, keep)), B
+
+
+@pytest.mark.parametrize("E,groups,keep", [(64, 32, 2), (64, 32, 5), (60, 30, 3), (64, 8, 4), (256, 8, 4), (512, 32, 3)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_biases_of_the_lowest_and_largest_value(E, groups, keep, score):
+    """The sum of two keys of +-3.4e38 leaves fp32, the order of the groups does not: a mask of the type's lowest
+    value puts experts last, but leaves them to choose from."""
+    x = make(60, E, E)
+    x[:20, ::3] = -INF
+    x[20:30, :E // 2] = -INF
+    size = E // groups
+    last, one, rest, top, mixed = (torch.zeros(E, device="cuda") for _ in range(5))
+    last[:E - size] = LOWEST                      # all but the last group
+    one[:] = LOWEST
+    one[E - 1] = 0.0                              # all but one expert
+    rest[size:] = LOWEST
+    rest[E // 2] = -INF
+    top[::size] = -LOWEST                         # the largest value
+    top[1::size] = -LOWEST
+    top[:size] = 0.0
+    mixed[::2] = LOWEST
+    mixed[1::4] = -LOWEST
+    for bias in (last, one, rest, top, mixed):
+        for k in (2, 6, 8, 9):
+            idx, w = ops.route_experts(x, k, score=score, bias=bias, n_groups=groups, top_groups=keep)
+            assert torch.equal(idx.long(), ro.choose(x, k, score, bias, groups, keep))
+            assert bool(torch.isfinite(w).all())
