@@ -793,6 +793,15 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
     route_one<T>(logits, a, t0 + (__ffs(open) - 1) / L, idx, weights);
 }
 
+// Exponential of the gradient for logits of type T.
+template <typename T>
+__device__ __forceinline__ float grad_exp(float v) {
+  if constexpr (std::is_same<T, float>::value)
+    return expf(v);
+  else
+    return fast_exp(v);
+}
+
 // d l from d w. With s the scores, w' the renormalised weights, G_e the sum of
 // scale dw over the slots that chose e and n_e their number:
 //   softmax, renormalised   dl_e = w'_e (G_e - n_e inner),           inner = sum_e w'_e G_e
@@ -850,9 +859,13 @@ __device__ __forceinline__ void store_span(T* __restrict__ row, int e0, int E, i
 
 // The slots' values go to their experts' lanes through shared memory: of the
 // slots that chose an expert the first adds up all of them, in slot order.
-// Exponentials and reciprocals are the approximate ones, within 2^-21. A lane
-// holds KS of its token's slots: one where k <= L, which leaves registers for
-// a fourth CTA per SM and cuts the slots' code by KS^2.
+// For 16-bit logits the exponentials are the approximate ones: an expert |v|
+// below the row's maximum is off by (4 + 1.5 |v|) 2^-24, which at |v| = 80,
+// where e^-v nearly leaves fp32, is 1.5% of fp16's half step and
+// 0.2% of bf16's. fp32 logits take expf (262,144 x 64, top-6: 63 us where the
+// approximate ones took 56). A lane holds KS of its token's slots: one where
+// k <= L, which leaves registers for a fourth CTA per SM and cuts the slots'
+// code by KS^2.
 //
 // Bound by issuing instructions, not by memory: 262,144 x 64 bf16, top-6,
 // takes 43.5 us (80 MB, 1.8 TB/s; 56.5 with four slots a lane throughout),
@@ -955,13 +968,13 @@ __global__ void __launch_bounds__(kRouteThreads)
     for (int j = 0; j < V; ++j) {
       rest[j] = 1.f;
       if (sigmoid) {
-        const float z = fast_exp(-fabsf(l[j]));
+        const float z = grad_exp<T>(-fabsf(l[j]));
         const float inv = fast_rcp(1.f + z);
         rest[j] = (l[j] > 0.f ? z : 1.f) * inv;
         // s = e^min(l, 0) / (1 + z); renormalised, e^-m times that, which does not underflow with all of them.
-        p[j] = a.renormalize ? fast_exp(fminf(l[j], 0.f) - m) * inv : (l[j] > 0.f ? 1.f : z) * inv;
+        p[j] = a.renormalize ? grad_exp<T>(fminf(l[j], 0.f) - m) * inv : (l[j] > 0.f ? 1.f : z) * inv;
       } else {
-        p[j] = l[j] != kNegInf ? fast_exp(l[j] - m) : 0.f;  // NaN stays
+        p[j] = l[j] != kNegInf ? grad_exp<T>(l[j] - m) : 0.f;  // NaN stays
       }
       if (l[j] == kNegInf || (a.renormalize && !(n[j] > 0.f))) p[j] = 0.f;
       total += a.renormalize ? n[j] * p[j] : p[j];

@@ -122,3 +122,40 @@ def test_biases_of_the_lowest_and_largest_value(E, groups, keep, score):
             idx, w = ops.route_experts(x, k, score=score, bias=bias, n_groups=groups, top_groups=keep)
             assert torch.equal(idx.long(), ro.choose(x, k, score, bias, groups, keep))
             assert bool(torch.isfinite(w).all())
+
+
+@pytest.mark.parametrize("score,renorm", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+@pytest.mark.parametrize("E,k", [(16, 3), (64, 6), (200, 8), (512, 32)])
+def test_gradient_of_fp32_logits_far_from_the_maximum(score, renorm, E, k):
+    """Experts up to 80 below the row's maximum keep fp32's relative accuracy. The logits are multiples of 2^-8, so
+    their differences are exact and what is left is counted here in u = 2^-24: an exponential (2 ulps: 4), a sum of E
+    terms (16 in a lane, 5 levels: 21, on top of the terms' 4), a reciprocal and products with it (1 each)."""
+    n, u = 400, 2.0 ** -24
+    g = gen(E)
+    x = -torch.randint(0, 80 * 256, (n, E), generator=g, device="cuda").float() / 256
+    x[:, 0] = 0.0
+    idx = (torch.rand(n, E - 1, generator=g, device="cuda").argsort(1)[:, :k] + 1).int()
+    dw = torch.randn(n, k, generator=g, device="cuda")
+    d = ops.route_experts_backward(dw, x, idx, score=score, renormalize=renorm)
+    l = x.double()
+    at = idx.long()
+    G = torch.zeros_like(l).scatter_(1, at, dw.double())
+    if renorm:
+        log = l if score == "softmax" else torch.nn.functional.logsigmoid(l)
+        s = torch.softmax(torch.full_like(l, -INF).scatter(1, at, log.gather(1, at)), 1)
+    else:
+        s = torch.softmax(l, 1) if score == "softmax" else torch.sigmoid(l)
+    rest = torch.sigmoid(-l) if score == "sigmoid" else torch.ones_like(l)
+    if score == "sigmoid" and not renorm:
+        ref, A = s * rest * G, torch.zeros_like(l[:, :1])
+        diff = G
+    else:
+        diff = G - (s * G).sum(1, keepdim=True)
+        if renorm:
+            diff = torch.zeros_like(l).scatter_(1, at, diff.gather(1, at))
+        ref, A = s * rest * diff, (s * G.abs()).sum(1, keepdim=True)
+    # s: 4 + 25 + 1 + 1; the inner sum: a product, 21 for its adds, 4, and the 25 + 2 of the division; G: the scale; the
+    # last subtraction and two products. sigmoid: 1 + z, its reciprocal (1 ulp: 2) and a product in s, and in 1 - s, with z
+    more = 6 + 10 if score == "sigmoid" else 0
+    tol = u * s * rest * ((31 + 3 + more) * diff.abs() + (53 + more) * A + G.abs()) + 2.0 ** -126
+    assert bool(((d.double() - ref).abs() <= tol).all()), float(((d.double() - ref).abs() / tol).max())
