@@ -1052,9 +1052,7 @@ cudaError_t route_t(const void* logits, const RouteArgs& a, int32_t* idx, float*
   int lanes, per;
   if (wide_shape(a, lanes, per)) {
     const T* x = static_cast<const T*>(logits);
-    if (lanes == 4)
-      return per <= 16 ? launch_wide<T, 4, 16>(x, a, per, idx, weights, stream)
-                       : launch_wide<T, 4, 32>(x, a, per, idx, weights, stream);
+    if (lanes == 4) return launch_wide<T, 4, 16>(x, a, per, idx, weights, stream);  // at most 64 experts
     if (lanes == 8)
       return per <= 8    ? launch_wide<T, 8, 8>(x, a, per, idx, weights, stream)
              : per <= 16 ? launch_wide<T, 8, 16>(x, a, per, idx, weights, stream)
