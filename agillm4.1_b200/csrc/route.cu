@@ -37,10 +37,12 @@
 //   counting. Where keys are too close to be told apart, those of the list,
 //   or the two that make a group's score, are formed again in fp64. Only rows
 //   with more than 32 keys at the border, or a NaN or infinite softmax, go
-//   through the other kernel's code, one by one. That case now takes 41 us: 71 MB at 1.7 TB/s, still bound by
-//   issuing (58% of the slots at 24 warps per SM). Two CTAs per SM with 128
-//   registers took 45 us, 16 lanes a token 48, 64 registers with the keys
-//   written over the logits 47. 262,144 x 64 bf16, top-6: 47 us.
+//   through the other kernel's code, one by one. That case now takes 39 us:
+//   71 MB at 1.8 TB/s. Neither memory nor the issue slots (58% taken) are full:
+//   the chain of a token's dependent steps bounds it, at the 24 warps per SM
+//   that fit. Two CTAs per SM with 128 registers took 45 us, 16 lanes a token
+//   48, 64 registers with the keys written over the logits 47. 262,144 x 64
+//   bf16, top-6: 47 us.
 //
 // Few tokens (64 x 14: 2.3 us on the device) cost a launch and one pass's
 // latency.
@@ -406,11 +408,14 @@ __device__ __forceinline__ void mark_if_ge(uint32_t& bits, float v, float bound,
       : "f"(v), "f"(bound), "r"(bit));
 }
 
+// CTAs per SM: as many as shared memory lets in (4 lanes take 59 KB a CTA, three
+// an SM, and gain 1% from the registers: 65,536 x 32 with groups 23.5 us
+// against 23.9) or, for 32 experts a lane, as registers do.
 // RAW: neither bias nor groups, the key is the logit. Otherwise the register
 // key is the approximate score (plus bias); the list holds exact logits where
 // there is no bias.
 template <typename T, int L, int V, bool RAW>
-__global__ void __launch_bounds__(kRouteThreads, V <= 16 ? 4 : 3)
+__global__ void __launch_bounds__(kRouteThreads, V <= 16 && L > 4 ? 4 : 3)
     route_wide_kernel(const T* __restrict__ logits, RouteArgs a, int per, int run, int32_t* __restrict__ idx,
                       float* __restrict__ weights) {
   using Smem = WideSmem<L, V>;
@@ -867,9 +872,9 @@ __device__ __forceinline__ void store_span(T* __restrict__ row, int e0, int E, i
 // k <= L, which leaves registers for a fourth CTA per SM and cuts the slots'
 // code by KS^2.
 //
-// Bound by issuing instructions, not by memory: 262,144 x 64 bf16, top-6,
-// takes 43.5 us (80 MB, 1.8 TB/s; 56.5 with four slots a lane throughout),
-// 49,151 x 64 10.4 us.
+// Bound by the latency of its steps at 32 warps per SM (60% of the issue slots
+// are taken), not by memory: 262,144 x 64 bf16, top-6, takes 43.5 us (80 MB,
+// 1.8 TB/s; 56.5 with four slots a lane throughout), 49,151 x 64 10.4 us.
 template <typename T, int L, int V, int KS>
 __global__ void __launch_bounds__(kRouteThreads)
     route_backward_kernel(const float* __restrict__ dw, const T* __restrict__ logits, const int32_t* __restrict__ idx,
