@@ -42,7 +42,7 @@ import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
-from . import ops
+from . import _lib, ops
 from ._lib import MoEKernelError
 
 
@@ -377,18 +377,25 @@ class _B200Forward:
             raise MoEKernelError(f"8-bit experts take bf16 or fp16 activations, not {flat.dtype}")
         (w1, b1, w2, b2), shared = self._fp8_weights(flat.device, flat.dtype)
         flat = flat.contiguous()
+        # The routed experts have an error word of their own.
+        err = torch.zeros(1, dtype=torch.int32, device=flat.device) if self.check_device_errors else None
         with torch.no_grad():
             logits_in = self.router(flat).float() if self.router_logits == "reference_gemm" else None
-            idx, gates, _, _ = ops.router_topk(flat, wr.detach().contiguous(), self.top_k, logits_in=logits_in)
+            idx, gates, _, _ = ops.router_topk(flat, wr.detach().contiguous(), self.top_k, logits_in=logits_in, err=err)
             add = None if residual is None else residual.contiguous()
             if shared:
                 x8 = ops.quantize_fp8(flat)
                 for v1, c1, v2, c2 in shared:
-                    h = ops.grouped_gemm_fp8(x8, v1, c1, relu=True, out_dtype=torch.float8_e4m3fn)
-                    y = ops.grouped_gemm_fp8(h, v2, c2, out_dtype=flat.dtype)
+                    h = ops.grouped_gemm_fp8(x8, v1, c1, relu=True, out_dtype=torch.float8_e4m3fn, err=err)
+                    y = ops.grouped_gemm_fp8(h, v2, c2, out_dtype=flat.dtype, err=err)
                     add = y if add is None else add + y
-            return ops.moe_experts_fp8(flat, idx, gates.float(), w1, b1, w2, b2, residual=add,
-                                       check_errors=self.check_device_errors)
+            out = ops.moe_experts_fp8(flat, idx, gates.float(), w1, b1, w2, b2, residual=add,
+                                      check_errors=self.check_device_errors)
+        if err is not None:
+            code = _lib.read_device_error(err)
+            if code:
+                raise MoEKernelError(f"device error word 0x{code:x} after the router and the shared experts")
+        return out
 
     # ---- expert streaming (agillm41.py:4367-4379, 7656-7668) ----
     def _host_expert_pack(self, dtype: torch.dtype):
