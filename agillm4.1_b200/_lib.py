@@ -117,6 +117,8 @@ SIGNATURES = {
     "agm_grouped_gemm_fp8": (_I, [_P, _P, _I64, _P, _P, _P, _I, _I, _I, _P, _P, _I, _I, _P, _I, _P, _P, _P]),
     "agm_moe_experts_fp8_workspace_bytes": (_SZ, [_I64, _I, _I, _I, _I]),
     "agm_moe_experts_fp8": (_I, [_P, _I, _I64, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "agm_moe_experts_fp8_shared": (_I, [_P, _I, _I64, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _SZ,
+                                        _P]),
     "agm_moe_aux_backward": (_I, [_P, _P, _I, _I64, _I, _I, _P, _SZ, _P, _P, _SZ, _I, _P]),
 }
 

@@ -6,6 +6,7 @@
 // columns of a row, whose four scales are one 32-bit word of the row's scale
 // tile.
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8.cuh"
 #include "kernels.h"
@@ -559,20 +560,24 @@ __global__ void __launch_bounds__(kThreads, 3) dispatch_rows_kernel(Fp8Dispatch 
 // ---------------------------------------------------------------------------
 // One warp per token and P x 256 columns: a lane sums P x 8 columns over the
 // token's rows, the loads of KU rows in flight at a time. ONE: k <= KU, so
-// that only one part's sums are held at a time. Bound by memory: 73,728 tokens
+// that only one part's sums are held at a time. SHARED: the outputs of shared
+// experts are there (their loop costs registers, with k <= 2 a CTA per SM and
+// 10 us at 73,728 tokens where there are none). Bound by memory: 73,728 tokens
 // x 1280 bf16, top-2, 567 MB in about 115 us, 4.9 TB/s. y comes rounded to T, as
 // the block in its own precision rounds it: fp32 would be 377 MB more to write
 // and 377 MB more to read here, some 115 us of 1.3 ms, for a relative error of
 // 0.0017 (the last rounding's) in place of 0.0023.
-template <typename T, int KU, int P, bool ONE>
+template <typename T, int KU, int P, bool ONE, bool SHARED>
 __global__ void __launch_bounds__(kThreads)
     combine_weighted_kernel(const T* __restrict__ y, const int32_t* __restrict__ row_of,
                             const float* __restrict__ weights, int64_t n, int nchunk, int k,
-                            const T* __restrict__ residual, T* __restrict__ out) {
+                            const T* __restrict__ residual, const T* __restrict__ shared, int n_shared,
+                            T* __restrict__ out) {
   static_assert(ONE || P == 1, "several parts only for few rows");
   const int lane = lane_id();
   const uint4* y4 = reinterpret_cast<const uint4*>(y);
   const uint4* res4 = reinterpret_cast<const uint4*>(residual);
+  const uint4* shared4 = reinterpret_cast<const uint4*>(shared);
   const int parts = (nchunk + 32 * P - 1) / (32 * P);
   const int64_t units = n * parts;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
@@ -601,6 +606,15 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] = 0.f;
       if (residual && c < nchunk) unpack8<T>(__ldcs(res4 + t * nchunk + c), acc);
+      if constexpr (SHARED) {
+#pragma unroll 1
+        for (int s = 0; s < n_shared && c < nchunk; ++s) {
+          float f[8];
+          unpack8<T>(__ldcs(shared4 + (s * n + t) * nchunk + c), f);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[j] += f[j];
+        }
+      }
     };
     auto add = [&](const uint4& v, float w) {
       float f[8];
@@ -742,27 +756,32 @@ cudaError_t dispatch_fp8(int dtype, const Fp8Dispatch& a, int num_sms, cudaStrea
 }
 
 cudaError_t combine_weighted(int dtype, const void* y, const int32_t* row_of, const float* weights, int64_t n, int d,
-                             int k, const void* residual, void* out, int num_sms, cudaStream_t stream) {
+                             int k, const void* residual, const void* shared, int n_shared, void* out, int num_sms,
+                             cudaStream_t stream) {
   const int nchunk = d / 8;
   auto launch = [&](auto kernel, int columns, auto zero) {
     using T = decltype(zero);
     return launch_kernel(kernel, dim3(warp_grid(n * ((nchunk + columns - 1) / columns), num_sms, 8)), dim3(kThreads), 0, stream,
                          static_cast<const T*>(y), row_of, weights, n, nchunk, k, static_cast<const T*>(residual),
-                         static_cast<T*>(out));
+                         static_cast<const T*>(shared), n_shared, static_cast<T*>(out));
   };
   // Few units: the narrowest, to use every SM. Many: enough loads in flight per warp.
-  auto pick = [&](auto zero) {
+  auto pick = [&](auto zero, auto with_shared) {
     using T = decltype(zero);
+    constexpr bool S = with_shared.value;
     const bool wide = n * ((nchunk + 31) / 32) >= static_cast<int64_t>(num_sms) * 64;
     if (k <= 2)
-      return wide ? launch(combine_weighted_kernel<T, 2, 5, true>, 160, zero)
-                  : launch(combine_weighted_kernel<T, 2, 1, true>, 32, zero);
+      return wide ? launch(combine_weighted_kernel<T, 2, 5, true, S>, 160, zero)
+                  : launch(combine_weighted_kernel<T, 2, 1, true, S>, 32, zero);
     if (k <= 4)
-      return wide ? launch(combine_weighted_kernel<T, 4, 2, true>, 64, zero)
-                  : launch(combine_weighted_kernel<T, 4, 1, true>, 32, zero);
-    return launch(combine_weighted_kernel<T, 8, 1, false>, 32, zero);
+      return wide ? launch(combine_weighted_kernel<T, 4, 2, true, S>, 64, zero)
+                  : launch(combine_weighted_kernel<T, 4, 1, true, S>, 32, zero);
+    return launch(combine_weighted_kernel<T, 8, 1, false, S>, 32, zero);
   };
-  return dtype == AGM_BF16 ? pick(__nv_bfloat16()) : pick(__half());
+  auto pick_dtype = [&](auto with_shared) {
+    return dtype == AGM_BF16 ? pick(__nv_bfloat16(), with_shared) : pick(__half(), with_shared);
+  };
+  return n_shared ? pick_dtype(std::true_type()) : pick_dtype(std::false_type());
 }
 
 }  // namespace agm

@@ -335,9 +335,10 @@ struct Fp8Dispatch {
   int n_zero;
 };
 cudaError_t dispatch_fp8(int dtype, const Fp8Dispatch& a, int num_sms, cudaStream_t stream);
-// out[t] = (residual[t] +) sum_r weights[t, r] y[row_of[t, r]], summed in fp32.
+// out[t] = (residual[t] +) sum_s shared[s, t] + sum_r weights[t, r] y[row_of[t, r]], summed in fp32.
 cudaError_t combine_weighted(int dtype, const void* y, const int32_t* row_of, const float* weights, int64_t n, int d,
-                             int k, const void* residual, void* out, int num_sms, cudaStream_t stream);
+                             int k, const void* residual, const void* shared, int n_shared, void* out, int num_sms,
+                             cudaStream_t stream);
 // c[r, :] = act(a[r, :] @ w[g]^T + bias[g]) over block-scaled e4m3 (fp8_gemm.cu).
 struct Fp8GemmArgs {
   const void* a = nullptr;         // e4m3 [a_rows, k]

@@ -226,7 +226,16 @@ size_t agm_moe_experts_fp8_workspace_bytes(int64_t n_tokens, int d, int n_expert
 int agm_moe_experts_fp8(const void* x, int dtype, int64_t n_tokens, int d, int n_experts, int top_k, int hidden,
                         const int32_t* idx, const float* weights, const void* w1, const void* s1, const float* b1,
                         const void* w2, const void* s2, const float* b2, const void* residual, void* out,
-                        void* workspace, size_t workspace_bytes, void* stream_) {
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  return agm_moe_experts_fp8_shared(x, dtype, n_tokens, d, n_experts, top_k, hidden, idx, weights, w1, s1, b1, w2, s2,
+                                    b2, residual, nullptr, 0, out, workspace, workspace_bytes, stream);
+}
+
+int agm_moe_experts_fp8_shared(const void* x, int dtype, int64_t n_tokens, int d, int n_experts, int top_k, int hidden,
+                               const int32_t* idx, const float* weights, const void* w1, const void* s1,
+                               const float* b1, const void* w2, const void* s2, const float* b2, const void* residual,
+                               const void* shared, int n_shared, void* out, void* workspace, size_t workspace_bytes,
+                               void* stream_) {
   if (dtype != AGM_BF16 && dtype != AGM_F16) return fail(AGM_ERR_UNSUPPORTED, "dtype must be AGM_BF16 or AGM_F16");
   if (n_tokens < 0) return fail(AGM_ERR_ARG, "n_tokens < 0");
   if (d <= 0 || d % 16 || hidden <= 0 || hidden % 16)
@@ -234,15 +243,16 @@ int agm_moe_experts_fp8(const void* x, int dtype, int64_t n_tokens, int d, int n
   if (n_experts < 1 || n_experts > AGM_ROUTE_MAX_EXPERTS)
     return fail(AGM_ERR_UNSUPPORTED, "number of experts must be in [1, 512]");
   if (top_k < 1 || top_k > AGM_ROUTE_MAX_TOPK) return fail(AGM_ERR_ARG, "top_k must be in [1, 32]");
+  if (n_shared < 0) return fail(AGM_ERR_ARG, "n_shared < 0");
   if (!workspace) return fail(AGM_ERR_ARG, "null pointer argument");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (n_tokens > INT32_MAX / top_k || segment_rows(n_tokens * top_k, n_experts) > INT32_MAX - 256)
     return fail(AGM_ERR_UNSUPPORTED, "too many rows for int32 indices");
   const ExpertsLayout L = carve(workspace, n_tokens, d, n_experts, top_k, hidden);
   if (L.bytes > workspace_bytes) return fail(AGM_ERR_WORKSPACE, "workspace too small");
-  if (n_tokens > 0 && (!x || !idx || !weights || !w1 || !s1 || !b1 || !w2 || !s2 || !b2 || !out))
+  if (n_tokens > 0 && (!x || !idx || !weights || !w1 || !s1 || !b1 || !w2 || !s2 || !b2 || !out || (n_shared && !shared)))
     return fail(AGM_ERR_ARG, "null pointer argument");
-  const void* ptrs[] = {x, w1, s1, b1, w2, s2, b2, residual, out, workspace};
+  const void* ptrs[] = {x, w1, s1, b1, w2, s2, b2, residual, shared, out, workspace};
   for (const void* p : ptrs)
     if (!aligned16(p)) return fail(AGM_ERR_ARG, "all tensors must be 16-byte aligned");
   if (n_tokens == 0) return done(cudaMemsetAsync(L.err, 0, sizeof(int), stream), "memset");
@@ -303,7 +313,8 @@ int agm_moe_experts_fp8(const void* x, int dtype, int64_t n_tokens, int d, int n
     e = agm::grouped_gemm_fp8(dtype, h, AGM_FP8_ROWS, sms, stream);
     if (e != cudaSuccess) return done(e, "grouped_gemm_fp8 fc2");
   }
-  return done(agm::combine_weighted(dtype, L.y, L.row_of, weights, n_tokens, d, top_k, residual, out, sms, stream),
+  return done(agm::combine_weighted(dtype, L.y, L.row_of, weights, n_tokens, d, top_k, residual, shared, n_shared, out,
+                                    sms, stream),
               "combine_weighted");
 }
 

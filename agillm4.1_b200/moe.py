@@ -371,7 +371,7 @@ class _B200Forward:
     def _forward_fp8(self, flat: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.Tensor:
         """The inference forward with 8-bit experts: the block's own router,
         then ops.moe_experts_fp8. Shared experts run as dense 8-bit products
-        and enter the weighted sum with the residual."""
+        and enter the weighted sum, which is rounded once, with the residual."""
         wr = self.router.weight
         if flat.dtype not in (torch.bfloat16, torch.float16):
             raise MoEKernelError(f"8-bit experts take bf16 or fp16 activations, not {flat.dtype}")
@@ -382,14 +382,15 @@ class _B200Forward:
         with torch.no_grad():
             logits_in = self.router(flat).float() if self.router_logits == "reference_gemm" else None
             idx, gates, _, _ = ops.router_topk(flat, wr.detach().contiguous(), self.top_k, logits_in=logits_in, err=err)
-            add = None if residual is None else residual.contiguous()
+            ys = None
             if shared:
                 x8 = ops.quantize_fp8(flat)
-                for v1, c1, v2, c2 in shared:
+                ys = flat.new_empty(len(shared), *flat.shape)
+                for y, (v1, c1, v2, c2) in zip(ys, shared):
                     h = ops.grouped_gemm_fp8(x8, v1, c1, relu=True, out_dtype=torch.float8_e4m3fn, err=err)
-                    y = ops.grouped_gemm_fp8(h, v2, c2, out_dtype=flat.dtype, err=err)
-                    add = y if add is None else add + y
-            out = ops.moe_experts_fp8(flat, idx, gates.float(), w1, b1, w2, b2, residual=add,
+                    ops.grouped_gemm_fp8(h, v2, c2, out_dtype=flat.dtype, out=y, err=err)
+            out = ops.moe_experts_fp8(flat, idx, gates.float(), w1, b1, w2, b2, shared=ys,
+                                      residual=None if residual is None else residual.contiguous(),
                                       check_errors=self.check_device_errors)
         if err is not None:
             code = _lib.read_device_error(err)

@@ -781,11 +781,13 @@ def grouped_gemm_fp8(a: FP8Tensor, w: FP8Tensor, bias: Optional[torch.Tensor] = 
 
 def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, w1: FP8Tensor, b1: torch.Tensor,
                     w2: FP8Tensor, b2: torch.Tensor, *, residual: Optional[torch.Tensor] = None,
-                    workspace: Optional[torch.Tensor] = None, check_errors: bool = False) -> torch.Tensor:
+                    workspace: Optional[torch.Tensor] = None, check_errors: bool = False,
+                    shared: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The routed experts of a MoE block with 8-bit weights:
-    out[t] = (residual[t] +) sum_r weights[t, r] * y(t, r), with
+    out[t] = (residual[t] +) (sum_s shared[s, t] +) sum_r weights[t, r] * y(t, r), with
     y(t, r) = W2[e] Q(relu(W1[e] Q(x[t]) + b1[e])) + b2[e], e = idx[t, r], and Q
     the quantisation of :func:`quantize_fp8`. y has x's dtype, sums are fp32.
+    ``shared`` [S, N, d] of x's dtype: the outputs of shared experts.
 
     x [N, d] bf16 or fp16; idx int32 [N, k] and weights fp32 [N, k], as
     :func:`route_experts` returns them (slots outside [0, E) contribute
@@ -809,16 +811,20 @@ def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, w
     _need("b2", b2, torch.float32, (E, d), dev)
     if residual is not None:
         _need("residual", residual, x.dtype, (n, d), dev)
+    n_shared = 0
+    if shared is not None:
+        n_shared = shared.shape[0] if shared.dim() else 0
+        _need("shared", shared, x.dtype, (n_shared, n, d), dev)
     if workspace is None:
         nbytes = int(lib.agm_moe_experts_fp8_workspace_bytes(n, d, E, k, H))
         workspace = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
     elif workspace.device != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise _lib.MoEKernelError(f"workspace must be a contiguous uint8 tensor on {dev}")
     out = torch.empty_like(x)
-    _call(dev, "agm_moe_experts_fp8", x.data_ptr(), dtype_code(x.dtype), n, d, E, k, H, idx.data_ptr(),
+    _call(dev, "agm_moe_experts_fp8_shared", x.data_ptr(), dtype_code(x.dtype), n, d, E, k, H, idx.data_ptr(),
           weights.data_ptr(), w1.q.data_ptr(), w1.scales.data_ptr(), b1.data_ptr(), w2.q.data_ptr(),
-          w2.scales.data_ptr(), b2.data_ptr(), _address(residual), out.data_ptr(), workspace.data_ptr(),
-          workspace.numel())
+          w2.scales.data_ptr(), b2.data_ptr(), _address(residual), _address(shared), n_shared, out.data_ptr(),
+          workspace.data_ptr(), workspace.numel())
     if check_errors:
         code = _lib.read_device_error(workspace[:4].view(torch.int32))
         if code:

@@ -584,6 +584,14 @@ AGM_API int agm_moe_experts_fp8(const void* x, int dtype, int64_t n_tokens, int 
                                 const float* b1, const void* w2, const void* s2, const float* b2,
                                 const void* residual, void* out, void* workspace, size_t workspace_bytes,
                                 void* stream);
+/* The same with the outputs of shared experts in the sum, which is rounded once:
+ *   out[t] = (residual[t] +) sum_s shared[s, t] + sum_r weights[t, r] * y(t, r)
+ *   shared [n_shared, n, d] (dtype), nullable where n_shared is 0 */
+AGM_API int agm_moe_experts_fp8_shared(const void* x, int dtype, int64_t n_tokens, int d, int n_experts, int top_k,
+                                       int hidden, const int32_t* idx, const float* weights, const void* w1,
+                                       const void* s1, const float* b1, const void* w2, const void* s2, const float* b2,
+                                       const void* residual, const void* shared, int n_shared, void* out,
+                                       void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
