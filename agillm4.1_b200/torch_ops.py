@@ -138,7 +138,7 @@ def moe_forward(x: torch.Tensor, w_router: torch.Tensor, w1: torch.Tensor, b1: t
 
 @moe_forward.register_fake
 def _(x, w_router, w1, b1, w2, b2, top_k, ws1=None, sb1=None, ws2=None, sb2=None):
-    return torch.empty_like(x)
+    return x.new_empty(x.shape)  # contiguous, whatever the strides of x
 
 
 @torch.library.custom_op(f"{_NS}::route_experts", mutates_args=())
@@ -222,7 +222,7 @@ def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, w
 
 @moe_experts_fp8.register_fake
 def _(x, idx, weights, w1, s1, b1, w2, s2, b2, residual):
-    return torch.empty_like(x)
+    return x.new_empty(x.shape)  # contiguous, whatever the strides of x
 
 
 __all__ = ["route_experts", "quantize_fp8", "quantize_fp8_weight", "dequantize_fp8", "grouped_gemm_fp8",
