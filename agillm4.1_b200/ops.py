@@ -584,9 +584,14 @@ def _need(what: str, t: torch.Tensor, dtype, shape, dev: torch.device) -> None:
     raise _lib.MoEKernelError(f"{what} must be contiguous")
 
 
+_INT_MAX = 2 ** 31 - 1  # widths, rows of a weight and k are ints of the C interface
+
+
 def _cuda_matrix(what: str, t: torch.Tensor, dim: int = 2) -> torch.device:
     """The GPU of a contiguous tensor of this many dimensions."""
     if t.is_cuda and t.dim() == dim and t.is_contiguous():
+        if t.numel() > _INT_MAX and max(t.shape[1:]) > _INT_MAX:
+            raise _lib.MoEKernelError(f"{what} must have at most 2^31 - 1 elements a row, not shape {tuple(t.shape)}")
         return t.device
     if t.dim() != dim:
         raise _lib.MoEKernelError(f"{what} must have {dim} dimensions, not shape {tuple(t.shape)}")
@@ -629,13 +634,16 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     :func:`agillm41_b200.route_experts` is the differentiable form."""
     dev = _cuda_matrix("logits", logits)
     n, E = logits.shape
+    top_groups = n_groups if top_groups is None else top_groups
+    if not (0 < top_k <= E and 0 < top_groups <= n_groups <= E):
+        raise _lib.MoEKernelError(f"top_k {top_k} must be in [1, {E}], top_groups {top_groups} in [1, n_groups] and "
+                                  f"n_groups {n_groups} in [1, {E}]")
     if bias is not None:
         _need("bias", bias, torch.float32, (E,), dev)
-    idx = torch.empty(n, max(top_k, 0), dtype=torch.int32, device=dev)
-    weights = torch.empty(n, max(top_k, 0), dtype=torch.float32, device=dev)
+    idx = torch.empty(n, top_k, dtype=torch.int32, device=dev)
+    weights = torch.empty(n, top_k, dtype=torch.float32, device=dev)
     _call(dev, "agm_route_experts", logits.data_ptr(), dtype_code(logits.dtype), n, E, top_k, _score_code(score),
-          _address(bias), n_groups, n_groups if top_groups is None else top_groups,
-          renormalize, scale, idx.data_ptr(), weights.data_ptr())
+          _address(bias), n_groups, top_groups, renormalize, scale, idx.data_ptr(), weights.data_ptr())
     return idx, weights
 
 
@@ -647,6 +655,8 @@ def route_experts_backward(dweights: torch.Tensor, logits: torch.Tensor, idx: to
     dev = _cuda_matrix("logits", logits)
     n, E = logits.shape
     k = idx.shape[-1] if idx.dim() else 0
+    if k > E:
+        raise _lib.MoEKernelError(f"idx has {k} slots a token for {E} experts")
     _need("idx", idx, torch.int32, (n, k), dev)
     _need("dweights", dweights, torch.float32, (n, k), dev)
     dlogits = torch.empty_like(logits)
@@ -805,6 +815,8 @@ def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, w
     if dw != d or w2.q.shape != (E, d, H):
         raise _lib.MoEKernelError(f"w1 {tuple(w1.q.shape)} and w2 {tuple(w2.q.shape)} do not fit x {tuple(x.shape)}")
     k = idx.shape[-1] if idx.dim() else 0
+    if k > _lib.AGM_ROUTE_MAX_TOPK:
+        raise _lib.MoEKernelError(f"idx has {k} slots a token, at most {_lib.AGM_ROUTE_MAX_TOPK} are served")
     _need("idx", idx, torch.int32, (n, k), dev)
     _need("weights", weights, torch.float32, (n, k), dev)
     _need("b1", b1, torch.float32, (E, H), dev)
