@@ -559,7 +559,7 @@ class _B200Forward:
         grad = torch.is_grad_enabled() and (flat.requires_grad or wr.requires_grad
                                             or any(p.requires_grad for p in params))
         if self.expert_precision == "fp8":
-            if grad or amp_mode:
+            if grad or amp_mode or (res is not None and res.requires_grad and torch.is_grad_enabled()):
                 raise MoEKernelError("8-bit experts run the inference forward only: call the module under "
                                      "torch.no_grad() and without autocast")
             if self.router_logits not in ("kernel", "reference_gemm"):

@@ -120,3 +120,15 @@ def test_shared_outputs_are_checked():
     for bad in (x, x[None].float(), x[None, :4], x[None].cpu(), torch.zeros(2, n, 2 * d, dtype=x.dtype, device="cuda")[:, :, ::2]):
         with pytest.raises(Error):
             ops.moe_experts_fp8(x, idx, w, w1, b1, w2, b2, shared=bad)
+
+
+def test_gradients_of_the_residual_are_refused_too():
+    """A frozen module and an input without gradient, but a residual with one: its gradient would be lost."""
+    m = module().requires_grad_(False)
+    x = torch.randn(20, 256, generator=gen(1), device="cuda").bfloat16()
+    res = torch.randn_like(x)
+    ref = m.forward_residual(x, res)
+    with pytest.raises(Error, match="no_grad"):
+        m.forward_residual(x, res.requires_grad_())
+    with torch.no_grad():
+        assert torch.equal(m.forward_residual(x, res), ref)
