@@ -259,8 +259,10 @@ class _B200Forward:
     #             (ops.moe_experts_fp8), from copies of the expert weights
     #             quantised when first used and again whenever a parameter
     #             changes (as its version counter tells: writes through
-    #             .data do not count). Routing stays as it is. bf16 and fp16
-    #             modules.
+    #             .data do not count; parameters made in inference mode have
+    #             no counter and are quantised in every call, which no
+    #             graph captures). The parameters stay as they are, beside the
+    #             copies. Routing stays as it is. bf16 and fp16 modules.
     expert_precision = "model"
 
     def _packed_weights(self, device: torch.device, dtype: torch.dtype):
@@ -348,6 +350,9 @@ class _B200Forward:
                 stream.wait_event(cache.made)
             return cache.pack
         if torch.cuda.is_current_stream_capturing():
+            if not counted:
+                raise MoEKernelError("parameters made in inference mode have no version counter, so their 8-bit copies are "
+                                     "made in every call, which cannot be captured: make the module outside of it")
             raise MoEKernelError("the 8-bit experts are not up to date: run the module once before capturing it")
         w1, b1, w2, b2, sh = packed
         groups = [(w1, b1, w2, b2)]

@@ -132,3 +132,16 @@ def test_gradients_of_the_residual_are_refused_too():
         m.forward_residual(x, res.requires_grad_())
     with torch.no_grad():
         assert torch.equal(m.forward_residual(x, res), ref)
+
+
+def test_parameters_made_in_inference_mode():
+    """They have no version counter: quantised in every call, and a capture is refused with that reason."""
+    with torch.inference_mode():
+        m = module()
+        x = torch.randn(20, 256, generator=gen(1), device="cuda").bfloat16()
+        first = m(x)
+        m.experts[0][0].weight.mul_(1.5)
+        assert not torch.equal(m(x), first)
+        with pytest.raises(Error, match="version counter"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                m(x)
