@@ -715,6 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto poll = [&]() {
         int v = lane == 0 ? ld_acquire_gpu(args.done + b) : 0;
         v = __shfl_sync(0xffffffffu, v, 0);
+        __syncwarp();  // a shuffle orders no memory, and the elected lane need not be the one that acquired
         if (v >= num_n0) {
           asm volatile("fence.proxy.async.global;" ::: "memory");
           ready = true;
