@@ -703,7 +703,9 @@ def _need_fp8(what: str, t: FP8Tensor, dim: int, dev: Optional[torch.device] = N
 def quantize_fp8(x: torch.Tensor) -> FP8Tensor:
     """Rows [rows, width] (width a multiple of 16) -> e4m3 with one power-of-two
     scale per 128 elements of a row: 2^p, p the least integer with
-    amax <= 448 * 2^p. NaN and infinities become NaN and do not count for amax."""
+    amax <= 448 * 2^p. NaN and infinities become NaN and do not count for amax.
+    Rounding may go up to the next power of two, which the largest values of a
+    type do not have: 65504 in fp16 stands for 65536."""
     dev = _cuda_matrix("x", x)
     rows, width = x.shape
     t = FP8Tensor(torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=dev),
@@ -729,7 +731,7 @@ def quantize_fp8_weight(w: torch.Tensor, *, out: Optional[FP8Tensor] = None) -> 
 
 
 def dequantize_fp8(t: FP8Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values an :class:`FP8Tensor` stands for, rounded once to ``dtype``."""
+    """The values an :class:`FP8Tensor` stands for, rounded once to ``dtype`` (to infinity past its range)."""
     dev = _need_fp8("t", t, 3 if isinstance(t, FP8Tensor) and t.q.dim() == 3 else 2)
     rows, width = t.q.shape[-2:]
     G = t.q.shape[0] if t.q.dim() == 3 else 1
@@ -756,7 +758,8 @@ def grouped_gemm_fp8(a: FP8Tensor, w: FP8Tensor, bias: Optional[torch.Tensor] = 
     belongs to the group.
 
     out_dtype: torch.bfloat16, torch.float16, or torch.float8_e4m3fn for an
-    FP8Tensor quantised from the fp32 results (the next product's input).
+    FP8Tensor quantised from the fp32 results (the next product's input), whose
+    scales are new: rows that are not written have scale bytes of 0.
     Segments that do not fit are left out and set the device error word ``err``."""
     dev = _need_fp8("a", a, 2)
     _need_fp8("w", w, 3, dev)

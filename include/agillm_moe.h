@@ -538,13 +538,15 @@ AGM_API int agm_route_experts_backward(const float* dweights, const void* logits
  * byte 16 * (r % 32) + 4 * (r % 128 / 32) + b % 4 of tile (r / 128, b / 4).
  * The exponent is the least p with max|x| <= 448 * 2^p (>= -127), values are
  * rounded to nearest even; NaN and infinities become NaN and do not count for
- * the maximum. width is a multiple of 16. */
+ * the maximum. Rounding may go up to the next power of two, which the largest
+ * values of a type do not have (65504 in fp16 stands for 65536). width is a
+ * multiple of 16. */
 AGM_API size_t agm_fp8_scale_bytes(int64_t rows, int width);
 AGM_API int agm_quantize_fp8(const void* x, int dtype, int64_t rows, int width, void* q, void* scales, void* stream);
 /* w [groups, n, width] -> q [groups, n, width], scales [groups][tiles of one matrix] */
 AGM_API int agm_quantize_fp8_weight(const void* w, int dtype, int64_t groups, int n, int width, void* q, void* scales,
                                     void* stream);
-/* q, scales -> out [groups, rows, width] (dtype): q * 2^p, rounded once. */
+/* q, scales -> out [groups, rows, width] (dtype): q * 2^p, rounded once (to infinity past the type's range). */
 AGM_API int agm_dequantize_fp8(const void* q, const void* scales, int64_t groups, int64_t rows, int width, int dtype,
                                void* out, void* stream);
 
