@@ -411,10 +411,18 @@ __device__ __forceinline__ void mark_if_ge(uint32_t& bits, float v, float bound,
 // CTAs per SM: as many as shared memory lets in (4 lanes take 59 KB a CTA, three
 // an SM, and gain 1% from the registers: 65,536 x 32 with groups 23.5 us
 // against 23.9) or, for 32 experts a lane, as registers do.
-// RAW: neither bias nor groups, the key is the logit. Otherwise the register
-// key is the approximate score (plus bias); the list holds exact logits where
-// there is no bias.
-template <typename T, int L, int V, bool RAW>
+//
+// KEYS: what orders the experts. kLogits: neither bias nor groups, the logit
+// itself. kGroupsThenLogits: groups without a bias; the register key is the
+// approximate score until the groups are chosen, then the logit, which orders
+// as the scores do, exactly, also where those of a confident row (or sigmoids
+// near zero) are below their error: 65,536 x 256 with logits of deviation 10
+// take 98 us, mostly for group scores in fp64, where a bound from the scores
+// let whole groups into the list and took 942; of deviation 1, 41 and 43.
+// kBiased: the register key is the approximate score plus bias.
+enum WideKeys { kLogits, kGroupsThenLogits, kBiased };
+
+template <typename T, int L, int V, WideKeys KEYS>
 __global__ void __launch_bounds__(kRouteThreads, V <= 16 && L > 4 ? 4 : 3)
     route_wide_kernel(const T* __restrict__ logits, RouteArgs a, int per, int run, int32_t* __restrict__ idx,
                       float* __restrict__ weights) {
@@ -429,8 +437,8 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 && L > 4 ? 4 : 3)
   const int E = a.n_experts;
   const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (kRouteThreads / 32) + warp_id()) * TOK;
   const int toks = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(TOK), a.n - t0)));
-  const bool grouped = !RAW && a.top_groups < a.n_groups;
-  const bool biased = !RAW && a.bias != nullptr;
+  constexpr bool RAW = KEYS == kLogits, BIASED = KEYS == kBiased;
+  const bool grouped = KEYS == kGroupsThenLogits || (BIASED && a.top_groups < a.n_groups);
   const bool sigmoid = a.score == AGM_ROUTE_SIGMOID;
   const float inv_per = 1.f / per;
   pdl_wait();
@@ -446,7 +454,7 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 && L > 4 ? 4 : 3)
       const int i = 128 * q + 4 * lane;
       f[q] = i / (L * V) < toks ? load4<T>(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    if (biased)
+    if constexpr (BIASED)
       for (int e = threadIdx.x; e < E; e += kRouteThreads) bias_s[e / V * LD + e % V] = a.bias[e];
 #pragma unroll
     for (int q = 0; q < N; ++q) {
@@ -461,7 +469,7 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 && L > 4 ? 4 : 3)
         const int c = owner(e, inv_per);
         sm.logit[k][c * LD + (e - c * per)] = Traits<T>::to_f(src[k * E + e]);
       }
-    if (biased)
+    if constexpr (BIASED)
       for (int e = threadIdx.x; e < E; e += kRouteThreads) {
         const int c = owner(e, inv_per);
         bias_s[c * LD + (e - c * per)] = a.bias[e];
@@ -512,7 +520,7 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 && L > 4 ? 4 : 3)
 #pragma unroll
         for (int j = 0; j < SB; ++j) s[j] = fast_exp(key[b * SB + j] - m) * inv_t;
       }
-      if (biased) {
+      if constexpr (BIASED) {
         if constexpr (SB % 4 == 0) {
 #pragma unroll
           for (int j = 0; j < SB; j += 4) {
@@ -601,7 +609,7 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 && L > 4 ? 4 : 3)
       while (pair) {
         const int j = __ffs(pair) - 1;
         pair &= pair - 1;
-        const double d = exact_score(my_logit[j], sigmoid, m, exact_t) + (biased ? bias_s[sub * LD + j] : 0.f);
+        const double d = exact_score(my_logit[j], sigmoid, m, exact_t) + (BIASED ? bias_s[sub * LD + j] : 0.f);
         e2 = fmax(e2, fmin(e1, d));
         e1 = fmax(e1, d);
       }
@@ -623,6 +631,21 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 && L > 4 ? 4 : 3)
     if (!kept)
 #pragma unroll
       for (int b = 0; b < 4; ++b) top[b] = kNegInf;
+  }
+  if constexpr (KEYS == kGroupsThenLogits) {
+    // NaN reaches neither a maximum nor a bound, -inf no bound.
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+      const float4 f = *reinterpret_cast<const float4*>(my_logit + 4 * q);
+      key[4 * q] = f.x, key[4 * q + 1] = f.y, key[4 * q + 2] = f.z, key[4 * q + 3] = f.w;
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      top[b] = kNegInf;
+#pragma unroll
+      for (int j = b * SB; j < (b + 1) * SB; ++j) top[b] = fmaxf(top[b], key[j]);
+      if (!kept) top[b] = kNegInf;
+    }
   }
   // 3. A bound that at least k keys reach: the k-th largest quarter maximum.
   order2(top[0], top[1]);
@@ -646,7 +669,7 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 && L > 4 ? 4 : 3)
 #pragma unroll
   for (int i = 1; i < 8; ++i) bound = i < a.k ? top[i] : bound;
   const float error = (sigmoid ? 10.f : 32.f) * 0x1p-24f;  // of (1 + |key|)
-  if (!RAW) bound -= 2.f * error * (1.f + fabsf(bound));
+  if (BIASED) bound -= 2.f * error * (1.f + fabsf(bound));
   if (!(bound > kNegInf)) bound = -FLT_MAX;
   // 4. The keys that reach it, in index order.
   uint32_t hit = 0;
@@ -667,11 +690,11 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 && L > 4 ? 4 : 3)
     const int j = __ffs(hit) - 1;
     hit &= hit - 1;
     sm.id[tok][at] = sub * per + j;
-    sm.key[tok][at] = RAW ? my_logit[j] + 0.f : __int_as_float(sub * LD + j);  // -0 = 0; or its place
+    sm.key[tok][at] = BIASED ? __int_as_float(sub * LD + j) : my_logit[j] + 0.f;  // its place; or -0 = 0
   }
   const int len = min(total, kWideList);
   const int len4 = (len + 3) & ~3;
-  if constexpr (RAW) {
+  if constexpr (!BIASED) {
     for (int i = len + sub; i < len4; i += L) sm.key[tok][i] = kNegInf;
   } else {
     // The keys again, shared out over the lanes: few hold most of the list.
@@ -681,10 +704,8 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 && L > 4 ? 4 : 3)
       if (i < len) {
         const int at = __float_as_int(sm.key[tok][i]);
         v = sm.logit[tok][at];
-        if (biased) {
-          v = sigmoid ? fast_rcp(1.f + fast_exp(-v)) : fast_exp(v - m) * inv_t;  // as in 2
-          v += bias_s[at];
-        }
+        v = sigmoid ? fast_rcp(1.f + fast_exp(-v)) : fast_exp(v - m) * inv_t;  // as in 2
+        v += bias_s[at];
       }
       sm.key[tok][i] = v + 0.f;  // -0 = 0
     }
@@ -696,7 +717,7 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 && L > 4 ? 4 : 3)
   for (int p = sub; p < len; p += L) {
     const float c = sm.key[tok][p];
     int above = 0;
-    if constexpr (RAW) {
+    if constexpr (!BIASED) {
       // Keys are exact: an equal one before p is above it too, o > c being o >= the float after c.
       const float up = __int_as_float(__float_as_int(c) + (c < 0.f ? -1 : 1));
       for (int q = 0; q < len4; q += 4) {
@@ -718,21 +739,21 @@ __global__ void __launch_bounds__(kRouteThreads, V <= 16 && L > 4 ? 4 : 3)
   __syncwarp();
   // Neighbours closer than the error of keys leave the order open; equal keys
   // leave a rank empty.
-  for (int r = sub; !RAW && r < a.k && r < len; r += L) {
+  for (int r = sub; BIASED && r < a.k && r < len; r += L) {
     const float c = sm.sorted[tok][r];
     const bool more = r + 1 < len;
     near |= sm.sel[tok][r] < 0 || (more && sm.sel[tok][r + 1] < 0) ||
-            (biased && more && c - sm.sorted[tok][r + 1] <= error * (1.f + fabsf(c)));
+            (more && c - sm.sorted[tok][r + 1] <= error * (1.f + fabsf(c)));
   }
-  if (!RAW && __any_sync(kAll, near && live)) {
-    if (biased) need_sum();
+  if (BIASED && __any_sync(kAll, near && live)) {
+    need_sum();
     near = (__ballot_sync(kAll, near) & part) != 0 && live;
     __syncwarp();
-    // Again with exact keys (the logits, where there is no bias), equal ones by index.
+    // Again with exact keys, equal ones by index.
     if (near)
       for (int p = sub; p < len; p += L) {
         const int e = sm.id[tok][p];
-        sm.exact[tok][p] = biased ? exact_score(sm.logit[tok][place(e)], sigmoid, m, exact_t) + a.bias[e] : sm.key[tok][p];
+        sm.exact[tok][p] = exact_score(sm.logit[tok][place(e)], sigmoid, m, exact_t) + a.bias[e];
       }
     __syncwarp();
     if (near)
@@ -1028,7 +1049,9 @@ cudaError_t launch_wide(const T* logits, const RouteArgs& a, int per, int32_t* i
                         cudaStream_t stream) {
   const int smem = static_cast<int>(sizeof(WideSmem<L, V>)) * (kRouteThreads / 32) + L * WideSmem<L, V>::kLane * 4;
   const int run = a.n_experts == L * V && reinterpret_cast<uintptr_t>(logits) % (4 * sizeof(T)) == 0;
-  const auto kernel = !a.bias && a.top_groups == a.n_groups ? route_wide_kernel<T, L, V, true> : route_wide_kernel<T, L, V, false>;
+  const auto kernel = a.bias                       ? route_wide_kernel<T, L, V, kBiased>
+                      : a.top_groups < a.n_groups ? route_wide_kernel<T, L, V, kGroupsThenLogits>
+                                                  : route_wide_kernel<T, L, V, kLogits>;
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
   const int64_t per_cta = kRouteThreads / L;
