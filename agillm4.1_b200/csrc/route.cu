@@ -206,6 +206,7 @@ __device__ __forceinline__ bool select_experts(const float (&l)[V], const RouteA
   uint32_t used = 0;
   F prev = F(INFINITY);
   float prev_l = 0.f, prev_b = 0.f;
+  bool same = false;  // the last two picks are equal in logit and bias
   const int picks = a.k + (inexact ? 1 : 0);
   for (int r = 0; r < picks; ++r) {
     F v = F(kNegInf);
@@ -225,7 +226,8 @@ __device__ __forceinline__ bool select_experts(const float (&l)[V], const RouteA
       const int src = (threadIdx.x & 31 & ~(L - 1)) | (id & (L - 1));
       vl = __shfl_sync(0xffffffffu, vl, any ? src : 0);
       const float vb = any ? a.bias[id] : 0.f;
-      if (any && r > 0 && prev - v <= F(1.9e-6f) * (F(1) + fabs(v)) && !(vl == prev_l && vb == prev_b)) near = true;
+      same = any && r > 0 && vl == prev_l && vb == prev_b;
+      if (any && r > 0 && prev - v <= F(1.9e-6f) * (F(1) + fabs(v)) && !same) near = true;
       prev = v;
       prev_l = vl;
       prev_b = vb;
@@ -236,6 +238,19 @@ __device__ __forceinline__ bool select_experts(const float (&l)[V], const RouteA
       for (int i = 0; i < KS; ++i)
         if (r == sub + L * i) sel[i] = id;
     }
+  }
+  if constexpr (kFast) {
+    // Equal experts on both sides of the border need no second look at one
+    // another, but hide a later one that fp32 takes for equal.
+    bool hidden = false;
+    if (same)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (!((used >> j) & 1u) && prev - key[j] <= F(1.9e-6f) * (F(1) + fabs(prev)) &&
+            !(l[j] == prev_l && a.bias[sub + L * j] == prev_b))
+          hidden = true;
+    const uint32_t token = L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1u) << (threadIdx.x & 31 & ~(L - 1));
+    near |= (__ballot_sync(0xffffffffu, hidden) & token) != 0;
   }
   return near;
 }

@@ -182,3 +182,21 @@ def test_confident_rows_with_groups(score, mul, off):
         return best
 
     assert time(x * mul + off) < 8 * time(x)          # 2.5 times, where it was 22 and 48
+
+
+@pytest.mark.parametrize("E,k", [(30, 4), (72, 15), (300, 9), (512, 32), (64, 8), (256, 8)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_equal_keys_at_the_border_hide_no_larger_one(E, k, score):
+    """More equal experts than slots, and one after them that is larger by less than fp32 can tell."""
+    x = torch.full((50, E), -9984.0, device="cuda")
+    first = torch.arange(k // 2, device="cuda")
+    x[:, first] = make(50, k // 2, E) + 2
+    late = E - 1 - torch.arange(50, device="cuda") % (E // 4)
+    x[torch.arange(50), late] = -20.0
+    x[25:, E // 2] = -21.0
+    for b in (torch.ones(E, device="cuda"), torch.zeros(E, device="cuda"), torch.full((E,), -3.0, device="cuda")):
+        for t in (x, x.bfloat16()):
+            idx, _ = ops.route_experts(t, k, score=score, bias=b)
+            ref = ro.choose(t, k, score, b)
+            assert torch.equal(idx.long(), ref)
+            assert bool((ref == late[:, None]).any(1).all())
