@@ -22,8 +22,9 @@
 //   128 columns per warp into registers at once and releases the shared
 //   columns first, so the next tile waits for that load and not for the
 //   epilogue's arithmetic. 147,456 rows over 14 groups: 1280 -> 3200 with
-//   e4m3 output 504 us (2.40 PFLOP/s), 3200 -> 1280 with bf16 output 480 us
-//   (2.52). A k-block of a pair takes 0.43 us, 0.28 when nothing is loaded:
+//   e4m3 output 507 us (2.38 PFLOP/s), 3200 -> 1280 with bf16 output 469 us
+//   (2.58), in runs of a few launches; back to back for seconds, under the 1 kW
+//   cap, 588 us (2.05) and 547 to 584 us (2.07 to 2.21). A k-block of a pair takes 0.43 us, 0.28 when nothing is loaded:
 //   what bounds it is the 64 KB that come from L2 meanwhile (11 TB/s over all
 //   SMs). A change of tiles adds 0.8 us. Three and four stages instead of five
 //   were 17% and 5% slower.

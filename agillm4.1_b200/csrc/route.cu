@@ -25,7 +25,9 @@
 // * route_kernel, any E <= 512, k <= 32 and grouping: L lanes hold a token's
 //   logits, V each (lane i holds experts i, i + L, ...) and pick k times the
 //   largest key. Few experts take few lanes, so a warp routes 8 tokens of a
-//   16-expert block; grouped routing takes the whole warp.
+//   16-expert block; grouped routing takes the whole warp. Its picks make large
+//   k slow where tokens are many: 65,536 x 256 without bias or groups take 94 us
+//   at k = 10, 134 at 16, 239 at 32 (25 at 8, on the kernel below).
 //
 // * route_wide_kernel, E >= 32 and k <= 8, bound by its instructions rather
 //   than by memory if it picked that way (65,536 x 256 grouped top-8 took 232
@@ -37,12 +39,12 @@
 //   counting. Where keys are too close to be told apart, those of the list,
 //   or the two that make a group's score, are formed again in fp64. Only rows
 //   with more than 32 keys at the border, or a NaN or infinite softmax, go
-//   through the other kernel's code, one by one. That case now takes 39 us:
-//   71 MB at 1.8 TB/s. Neither memory nor the issue slots (58% taken) are full:
+//   through the other kernel's code, one by one. That case now takes 37 us:
+//   71 MB at 1.9 TB/s. Neither memory nor the issue slots (60% taken) are full:
 //   the chain of a token's dependent steps bounds it, at the 24 warps per SM
 //   that fit. Two CTAs per SM with 128 registers took 45 us, 16 lanes a token
 //   48, 64 registers with the keys written over the logits 47. 262,144 x 64
-//   bf16, top-6: 47 us.
+//   bf16, top-6: 45 us.
 //
 // Few tokens (64 x 14: 2.3 us on the device) cost a launch and one pass's
 // latency.
@@ -909,8 +911,9 @@ __device__ __forceinline__ void store_span(T* __restrict__ row, int e0, int E, i
 // code by KS^2.
 //
 // Bound by the latency of its steps at 32 warps per SM (60% of the issue slots
-// are taken), not by memory: 262,144 x 64 bf16, top-6, takes 43.5 us (80 MB,
-// 1.8 TB/s; 56.5 with four slots a lane throughout), 49,151 x 64 10.4 us.
+// are taken), not by memory: 262,144 x 64 bf16, top-6, takes 42 us, 45
+// renormalised (80 MB, 1.9 TB/s; with four slots a lane throughout a quarter
+// more), 49,151 x 64 10.5 us.
 template <typename T, int L, int V, int KS>
 __global__ void __launch_bounds__(kRouteThreads)
     route_backward_kernel(const float* __restrict__ dw, const T* __restrict__ logits, const int32_t* __restrict__ idx,
