@@ -788,7 +788,8 @@ def grouped_gemm_fp8(a: FP8Tensor, w: FP8Tensor, bias: Optional[torch.Tensor] = 
         _need("out", out, out_dtype, (R, N), dev)
     _call(dev, "agm_grouped_gemm_fp8", a.q.data_ptr(), a.scales.data_ptr(), R, w.q.data_ptr(), w.scales.data_ptr(),
           _address(bias), G, N, K, _address(seg_start), _address(counts), relu, mode, out.data_ptr(),
-          0 if scales is not None else dtype_code(out_dtype), _address(scales), _address(err))
+          _lib.AGM_BF16 if scales is not None else dtype_code(out_dtype),  # no rows, no scales: it must be a type
+          _address(scales), _address(err))
     return out if scales is None else FP8Tensor(out, scales)
 
 

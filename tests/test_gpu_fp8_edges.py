@@ -54,3 +54,21 @@ def test_e4m3_products_into_a_given_tensor():
     raw = out.view(torch.uint8)
     assert bool((raw[128:256] == 5).all()) and bool((raw[384:] == 5).all()) and not bool(raw[100:128].any())
     assert not bool(y.scales[1].any()) and not bool(y.scales[3].any()) and bool(y.scales[2].any())
+
+
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float16, torch.float8_e4m3fn])
+def test_products_without_rows(out_dtype):
+    w = ops.quantize_fp8_weight(torch.randn(2, 32, 64, device="cuda"))
+    a = ops.quantize_fp8(torch.empty(0, 64, device="cuda"))
+    seg, cnt = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    y = ops.grouped_gemm_fp8(a, w, seg_start=seg, counts=cnt, out_dtype=out_dtype)
+    one = ops.FP8Tensor(w.q[:1].contiguous(), w.scales[:1].contiguous())
+    z = ops.grouped_gemm_fp8(a, one, out_dtype=out_dtype)
+    for t in (y, z):
+        if out_dtype == torch.float8_e4m3fn:
+            assert t.q.shape == (0, 32) and t.scales.shape == (0, 1, 512)
+            assert ops.dequantize_fp8(t).shape == (0, 32)
+        else:
+            assert t.shape == (0, 32)
+    none = ops.quantize_fp8_weight(torch.empty(0, 32, 64, device="cuda"))
+    assert none.q.shape == (0, 32, 64) and ops.dequantize_fp8(none).shape == (0, 32, 64)

@@ -145,3 +145,34 @@ def test_parameters_made_in_inference_mode():
         with pytest.raises(Error, match="version counter"):
             with torch.cuda.graph(torch.cuda.CUDAGraph()):
                 m(x)
+
+
+def test_no_tokens_with_shared_experts():
+    m = module()
+    m.check_device_errors = True
+    x = torch.empty(0, 256, dtype=torch.bfloat16, device="cuda")
+    with torch.no_grad():
+        assert m(x).shape == (0, 256) and m.forward_residual(x, x).shape == (0, 256)
+
+
+@pytest.mark.parametrize("k", [1, 2, 3, 4, 6])
+@pytest.mark.parametrize("n,d", [(50, 272), (12000, 256), (2500, 1296)])
+def test_shared_outputs_in_every_form_of_the_sum(n, d, k):
+    """Few and many tokens, one and several parts of a row: shared outputs of zeros change nothing, and without routed
+    rows the sum is the fp32 one of residual and shared outputs, rounded once."""
+    E, H, dtype = 5, 128, torch.float16
+    w1 = ops.quantize_fp8_weight(torch.randn(E, H, d, generator=gen(1), device="cuda") * d ** -0.5)
+    w2 = ops.quantize_fp8_weight(torch.randn(E, d, H, generator=gen(2), device="cuda") * H ** -0.5)
+    rest = (w1, torch.zeros(E, H, device="cuda"), w2, torch.ones(E, d, device="cuda"))
+    x = torch.randn(n, d, generator=gen(3), device="cuda").to(dtype)
+    idx = torch.randint(0, E, (n, k), generator=gen(4), device="cuda", dtype=torch.int32)
+    w = torch.randn(n, k, generator=gen(5), device="cuda")
+    sh = torch.randn(3, n, d, generator=gen(6), device="cuda").to(dtype) * 30
+    plain = ops.moe_experts_fp8(x, idx, w, *rest, residual=x)
+    assert torch.equal(ops.moe_experts_fp8(x, idx, w, *rest, residual=x, shared=torch.zeros_like(sh)), plain)
+    assert not torch.equal(ops.moe_experts_fp8(x, idx, w, *rest, residual=x, shared=sh), plain)
+    none = torch.full_like(idx, -1)
+    got = ops.moe_experts_fp8(x, none, w, *rest, residual=x, shared=sh)
+    assert torch.equal(got, (((x.float() + sh[0].float()) + sh[1].float()) + sh[2].float()).to(dtype))
+    got = ops.moe_experts_fp8(x, none, w, *rest, shared=sh[:1].contiguous())
+    assert torch.equal(got, sh[0])
